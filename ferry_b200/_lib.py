@@ -67,6 +67,28 @@ class LayerStats(ctypes.Structure):
         ('kernel_us', _dbl * 9), ('kernel_launches', _i64 * 9), ('hit_gemm_kernel_bytes', _i64)]
 
 
+class RouteArgs(ctypes.Structure):
+    """ferryb_route_args (include/ferryb.h)."""
+    _fields_ = [('logits', _vp), ('tokens', _i64), ('row_stride', _i64)] + [(n, _i32c) for n in (
+        'experts', 'topk', 'n_group', 'topk_group', 'logits_type', 'weights_type', 'score',
+        'group_score', 'norm_topk')] + [('scaling', ctypes.c_float)] + [(n, _vp) for n in (
+            'bias', 'selected', 'weights')]
+
+
+class Mxfp4ExpertsArgs(ctypes.Structure):
+    """ferryb_mxfp4_experts_args (include/ferryb.h)."""
+    _fields_ = [('cache', _vp), ('cache_slots', _i64), ('input', _vp), ('n_input', _i64),
+                ('input_stride', _i64), ('routing_weights', _vp), ('topk', _i64),
+                ('weights_type', _i32c), ('reserved', _i32c), ('slots', _vp), ('starts', _vp),
+                ('n_groups', _i64), ('rows', _vp), ('cols', _vp), ('routes', _i64), ('hidden', _i64),
+                ('intermediate', _i64), ('out', _vp), ('workspace', _vp), ('workspace_bytes', _i64),
+                ('err', _vp)]
+
+
+# element types of the C ABI (FERRYB_BF16 and so on, include/ferryb.h)
+ELEMENT_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
 # name -> (restype, argtypes); every symbol declared in include/ferryb.h.
 SIGNATURES = {
     'ferryb_last_error': (ctypes.c_char_p, []),
@@ -79,6 +101,11 @@ SIGNATURES = {
     'ferryb_execute_experts_noalloc_limit': (_i64, []),
     'ferryb_execute_experts_noalloc': (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp,
                                               _vp, _i64, _i64, _vp, _vp]),
+    'ferryb_route_experts': (_i32, [ctypes.POINTER(RouteArgs), _vp]),
+    'ferryb_quantize_mxfp4': (_i32, [_vp, _i32c, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp]),
+    'ferryb_dequantize_mxfp4': (_i32, [_vp, _i64, _vp, _i64, _i64, _i64, _vp, _i32c, _i64, _vp]),
+    'ferryb_execute_experts_mxfp4_workspace': (_i64, [_i64, _i64, _i64, _i64]),
+    'ferryb_execute_experts_mxfp4': (_i32, [ctypes.POINTER(Mxfp4ExpertsArgs), _vp]),
     'ferryb_plan_layer': (_i32, [ctypes.POINTER(Planner), _i64, _i32c, _vp, _i32c, _i32c, _vp, _vp,
                                  _vp, _i32c, _vp, _vp, _vp, _vp, _vp, _vp]),
     'ferryb_greedy_quota_rows': (_i32, [_i32c, _vp, _vp, _i32c, _vp, _i32c, _i32c, _vp, _vp, _vp]),

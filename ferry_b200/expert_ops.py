@@ -3,6 +3,14 @@
 and error behaviour (RuntimeError on bad input), backed by libferryb's sm_100a
 kernels through the C ABI.  Outputs are allocated by the torch caching
 allocator; inputs are borrowed.
+
+Beside them, operators the reference has no counterpart of: route_experts
+(softmax or sigmoid routers with a balance bias and groups),
+quantize_mxfp4 / dequantize_mxfp4 (4-bit weight rows) and
+execute_experts_mxfp4 (the routed experts over such rows).  They run on the
+device and current stream of their tensors, allocate only their outputs and
+workspace, and neither copy to the host nor wait for the GPU, so they can be
+captured into a CUDA graph.
 """
 import ctypes
 
@@ -127,6 +135,227 @@ def scatter_returned(returned, send_idx, tokens):
     call('ferryb_scatter_returned', ptr(ret), ptr(idx), ret.shape[0], tokens, hidden, ptr(out),
          ptr(ws), ws_bytes, stream_ptr(returned.device))
     return out.to(returned.dtype)
+
+
+def _cuda_call(device, name, *args):
+    """call() on `device`'s current stream, whatever the current device is."""
+    stream = stream_ptr(device)
+    if device.index == torch.cuda.current_device():
+        call(name, *args, stream)
+    else:
+        with torch.cuda.device(device):
+            call(name, *args, stream)
+
+
+def _same_device(device, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise _lib.FerrybError(f'{name} is on {t.device}, expected {device}')
+
+
+def _dense_rows(t):
+    """t itself if the values of a row are adjacent, else a contiguous copy."""
+    return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+SCORES = {'softmax': 0, 'sigmoid': 1}
+GROUP_SCORES = {'max': 0, 'top2': 1}
+
+
+def route_experts(logits, topk, *, score='softmax', bias=None, n_group=1, topk_group=1,
+                  group_score='max', norm_topk_prob=True, scaling=1.0, weights_dtype=BF16):
+    """Top-k routing from router logits [tokens, experts] (bf16, fp16 or
+    float32): (selected int64 [tokens, topk], weights [tokens, topk]), as
+    OffloadRuntime.execute takes them.
+
+    The scores are softmax(logits) or sigmoid(logits) (`score`); `bias`
+    (float32 [experts]) is added for the selection only.  With n_group > 1,
+    groups of consecutive experts, the topk_group groups of the largest
+    biased score (group_score 'max') or sum of their two largest ('top2')
+    stay.  The topk largest biased scores are selected, descending, ties to
+    the lower id.  The weights are the unbiased scores, divided by their sum
+    with norm_topk_prob, times `scaling`.  -inf logits mask experts with
+    softmax (a row of nothing else has weights 0); NaN scores are taken last
+    and give NaN weights.  Scores are compared in 64 bits.  At most 1024
+    experts, topk <= 32, n_group <= 32."""
+    require_cuda(logits, bias)
+    _check(logits.dim() == 2 and logits.dtype in _lib.ELEMENT_TYPES,
+           'logits must be bf16, fp16 or float32 [tokens, experts]')
+    _check(score in SCORES, f'score must be one of {sorted(SCORES)}')
+    _check(group_score in GROUP_SCORES, f'group_score must be one of {sorted(GROUP_SCORES)}')
+    _check(weights_dtype in _lib.ELEMENT_TYPES, 'weights_dtype must be bf16, fp16 or float32')
+    tokens, experts = logits.shape
+    dev = logits.device
+    if bias is not None:
+        _check(bias.dtype == torch.float32 and bias.shape == (experts,), 'bias must be float32 [experts]')
+        _same_device(dev, bias=bias)
+        bias = bias.contiguous()
+    logits = _dense_rows(logits)
+    if tokens > 1 and logits.stride(0) < experts:
+        logits = logits.contiguous()
+    topk = int(topk)
+    _check(0 < topk <= experts, f'topk must be in [1, {experts}]')
+    selected = torch.empty((tokens, topk), dtype=torch.int64, device=dev)
+    weights = torch.empty((tokens, topk), dtype=weights_dtype, device=dev)
+    args = _lib.RouteArgs(logits.data_ptr(), tokens, logits.stride(0), experts, topk, int(n_group),
+                          int(topk_group), _lib.ELEMENT_TYPES[logits.dtype],
+                          _lib.ELEMENT_TYPES[weights_dtype], SCORES[score], GROUP_SCORES[group_score],
+                          int(bool(norm_topk_prob)), float(scaling), _lib.addr(bias),
+                          selected.data_ptr(), weights.data_ptr())
+    _cuda_call(dev, 'ferryb_route_experts', ctypes.byref(args))
+    return selected, weights
+
+
+def _rows_2d(t, name):
+    """t as [rows, width] without a copy, the values of a row adjacent."""
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise _lib.FerrybError(f'{name}: the values of a row must be adjacent')
+    try:
+        t = t.view(-1, t.shape[-1]) if t.dim() != 2 else t
+    except RuntimeError:
+        raise _lib.FerrybError(f'{name}: the rows must be evenly spaced') from None
+    if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        raise _lib.FerrybError(f'{name}: rows overlap')
+    return t
+
+
+def _mxfp4_out(out, shape, device):
+    """(codes, scales) for values of `shape`: `out` checked, or new tensors."""
+    lead, width = tuple(shape[:-1]), shape[-1]
+    if out is None:
+        return (torch.empty(lead + (width // 2,), dtype=torch.uint8, device=device),
+                torch.empty(lead + (width // 32,), dtype=torch.uint8, device=device))
+    codes, scales = out
+    for name, t, n in (('codes', codes, width // 2), ('scales', scales, width // 32)):
+        _check(t.dtype == torch.uint8 and tuple(t.shape) == lead + (n,),
+               f'{name} must be uint8 {list(lead + (n,))}, got {t.dtype} {list(t.shape)}')
+        _same_device(device, **{name: t})
+    return codes, scales
+
+
+def quantize_mxfp4(x, out=None):
+    """MXFP4 of the last dimension of x (bf16, fp16 or float32, a multiple of
+    32 values): (codes uint8 [..., width / 2], scales uint8 [..., width / 32]).
+
+    Every 32 values share a power of two 2^(s - 127), s = the float32 exponent
+    field of their largest magnitude minus 2 (at least 0); a code is the value
+    over it, rounded half to even to {0, 0.5, 1, 1.5, 2, 3, 4, 6} and a sign,
+    two codes a byte, the lower nibble first.  A block holding an infinity or
+    a NaN has s = 255 and reads back as NaN.  `out`: (codes, scales) to write
+    to, such as the two parts of expert rows (ferry_b200.model.mxfp4_parts)."""
+    require_cuda(x)
+    _check(x.dim() >= 1 and x.dtype in _lib.ELEMENT_TYPES, 'x must be bf16, fp16 or float32')
+    width = x.shape[-1]
+    _check(width % 32 == 0, f'the last dimension ({width}) must be a multiple of 32')
+    codes, scales = _mxfp4_out(out, x.shape, x.device)
+    if x.numel() == 0:
+        return codes, scales
+    x2 = _dense_rows(x).reshape(-1, width)
+    if x2.shape[0] > 1 and x2.stride(0) < width:
+        x2 = x2.contiguous()
+    c2, s2 = _rows_2d(codes, 'codes'), _rows_2d(scales, 'scales')
+    _cuda_call(x.device, 'ferryb_quantize_mxfp4', ptr(x2), _lib.ELEMENT_TYPES[x.dtype], x2.shape[0], width,
+               x2.stride(0), ptr(c2), c2.stride(0), ptr(s2), s2.stride(0))
+    return codes, scales
+
+
+def dequantize_mxfp4(codes, scales, dtype=BF16, out=None):
+    """The values of quantize_mxfp4's codes and scales, rounded once to `dtype`
+    (bf16 and float32 hold them exactly, but for 6 * 2^127 and its like)."""
+    require_cuda(codes, scales, out)
+    _check(codes.dim() >= 1 and codes.dtype == torch.uint8 and scales.dtype == torch.uint8,
+           'codes and scales must be uint8')
+    lead, width = tuple(codes.shape[:-1]), 2 * codes.shape[-1]
+    _check(width % 32 == 0 and tuple(scales.shape) == lead + (width // 32,),
+           f'codes {list(codes.shape)} need scales {list(lead + (width // 32,))} (blocks of 32 values), '
+           f'got {list(scales.shape)}')
+    _check(dtype in _lib.ELEMENT_TYPES, 'dtype must be bf16, fp16 or float32')
+    _same_device(codes.device, scales=scales, out=out)
+    if out is None:
+        out = torch.empty(lead + (width,), dtype=dtype, device=codes.device)
+    _check(out.dtype == dtype and tuple(out.shape) == lead + (width,),
+           f'out must be {dtype} {list(lead + (width,))}')
+    if out.numel() == 0:
+        return out
+    o2 = _rows_2d(out, 'out')
+    c2, s2 = (_dense_rows(t).reshape(-1, t.shape[-1]) for t in (codes, scales))
+    c2, s2 = (t if t.shape[0] <= 1 or t.stride(0) >= t.shape[1] else t.contiguous() for t in (c2, s2))
+    _cuda_call(codes.device, 'ferryb_dequantize_mxfp4', ptr(c2), c2.stride(0), ptr(s2), s2.stride(0),
+               o2.shape[0], width, ptr(o2), _lib.ELEMENT_TYPES[dtype], o2.stride(0))
+    return out
+
+
+def execute_experts_mxfp4(cache, input, routing_weights, slots, starts, rows, cols, hidden, intermediate,
+                          *, out=None, err=None):
+    """execute_experts over MXFP4 expert rows: bf16 [routes, hidden], row p of
+    group g = (silu(x Wg^T) * (x Wu^T)) Wd^T * routing_weights[rows[p],
+    cols[p]] with x = input[rows[p]] and the weights of cache row slots[g].
+
+    cache: uint8 [slots, model.mxfp4_row_bytes(hidden, intermediate)], rows
+    as model.pack_expert_mxfp4 makes them.  Group g is the routes [starts[g],
+    starts[g + 1]): slots [G], starts [G + 1], rows and cols [routes] are
+    int64 CUDA tensors (LayoutBuffers' starts, rows and cols, for instance);
+    groups may be empty, and rows of `out` outside [starts[0], starts[G]) are
+    left as they were.  input is bf16, routing_weights [tokens, topk] bf16,
+    fp16 or float32.  hidden and intermediate are multiples of 128.
+
+    Sums, gate and up are float32; the activation and the result are rounded
+    to bf16 once each.  Index errors are found on the device: the routes'
+    rows become NaN (starts out of order: no row is written).  Without `err`
+    the call waits for the GPU and raises; with `err`, an int32 [1] CUDA tensor
+    that starts at 0, it returns at once and leaves a non-zero code there for
+    the caller to check, and can be captured into a CUDA graph."""
+    require_cuda(cache, input, routing_weights, slots, starts, rows, cols, out, err)
+    hidden, intermediate = int(hidden), int(intermediate)
+    _check(hidden > 0 and intermediate > 0 and hidden % 128 == 0 and intermediate % 128 == 0,
+           f'hidden ({hidden}) and intermediate ({intermediate}) must be multiples of 128')
+    dev = input.device
+    _same_device(dev, cache=cache, routing_weights=routing_weights, slots=slots, starts=starts, rows=rows,
+                 cols=cols, out=out, err=err)
+    row_bytes = 3 * hidden * intermediate // 32 * 17
+    _check(cache.dtype == torch.uint8 and cache.dim() == 2 and cache.shape[1] == row_bytes
+           and cache.is_contiguous() and cache.data_ptr() % 16 == 0,
+           f'cache must be contiguous 16-byte aligned uint8 [slots, {row_bytes}]')
+    _check(input.dtype == BF16 and input.dim() == 2 and input.shape[1] == hidden,
+           f'input must be bf16 [n, {hidden}]')
+    _check(routing_weights.dim() == 2 and routing_weights.shape[0] == input.shape[0]
+           and routing_weights.dtype in _lib.ELEMENT_TYPES,
+           'routing_weights must be bf16, fp16 or float32 [n, topk]')
+    for name, t in (('slots', slots), ('starts', starts), ('rows', rows), ('cols', cols)):
+        _check(t.dtype == torch.int64 and t.dim() == 1, f'{name} must be a 1-D int64 tensor')
+    groups, routes = slots.shape[0], rows.shape[0]
+    _check(starts.shape[0] == groups + 1, f'starts must have {groups + 1} entries (one more than slots)')
+    _check(cols.shape[0] == routes, 'rows and cols must have equal length')
+    if out is None:
+        out = torch.empty((routes, hidden), dtype=BF16, device=dev)
+    _check(out.dtype == BF16 and tuple(out.shape) == (routes, hidden) and out.is_contiguous(),
+           f'out must be contiguous bf16 [{routes}, {hidden}]')
+    wait = err is None
+    if not wait:
+        _check(err.dtype == torch.int32 and err.numel() == 1, 'err must be an int32 tensor of one element')
+    if routes == 0 or groups == 0:
+        return out
+    _check(cache.shape[0] > 0, 'cache has no slots')
+    if input.stride(1) != 1 or input.data_ptr() % 16 or (input.shape[0] > 1 and (
+            input.stride(0) % 8 or input.stride(0) < hidden)):
+        input = input.clone(memory_format=torch.contiguous_format)
+    routing_weights = routing_weights.contiguous()
+    slots, starts, rows, cols = (t.contiguous() for t in (slots, starts, rows, cols))
+    ws_bytes = _lib.lib().ferryb_execute_experts_mxfp4_workspace(routes, groups, hidden, intermediate)
+    if ws_bytes < 0:
+        raise _lib.FerrybError(_lib.lib().ferryb_last_error().decode())
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    if wait:
+        err = torch.zeros(1, dtype=torch.int32, device=dev)
+    args = _lib.Mxfp4ExpertsArgs(
+        cache.data_ptr(), cache.shape[0], input.data_ptr(), input.shape[0], input.stride(0),
+        routing_weights.data_ptr(), routing_weights.shape[1], _lib.ELEMENT_TYPES[routing_weights.dtype], 0,
+        slots.data_ptr(), starts.data_ptr(), groups, rows.data_ptr(), cols.data_ptr(), routes, hidden,
+        intermediate, out.data_ptr(), ws.data_ptr(), ws_bytes, err.data_ptr())
+    _cuda_call(dev, 'ferryb_execute_experts_mxfp4', ctypes.byref(args))
+    if wait:
+        _lib.check_device_error(err, 'execute_experts_mxfp4')
+    return out
 
 
 class H2DEngine:

@@ -71,6 +71,31 @@ def pack_expert(gate_w, up_w, down_w):
     return torch.cat([gate_w.reshape(-1), up_w.reshape(-1), down_w.reshape(-1)]).to(torch.bfloat16)
 
 
+def mxfp4_row_bytes(hidden, intermediate):
+    """Bytes of an expert row in MXFP4: 3 * H * I codes of half a byte, then one
+    scale byte for every 32 of them (17 bytes where a bf16 row has 64)."""
+    return 3 * hidden * intermediate // 32 * 17
+
+
+def mxfp4_parts(rows):
+    """(codes, scales) of MXFP4 expert rows [..., mxfp4_row_bytes]: views of the
+    rows, as ferry_b200.expert_ops.quantize_mxfp4 and dequantize_mxfp4 take
+    them.  The codes are in the order of pack_expert's values."""
+    split = rows.shape[-1] // 17 * 16
+    return rows[..., :split], rows[..., split:]
+
+
+def pack_expert_mxfp4(gate_w, up_w, down_w):
+    """One expert (CUDA nn.Linear weights) as an MXFP4 row: pack_expert's row
+    quantised in blocks of 32 along H (gate, up) and I (down).  H and I are
+    multiples of 32."""
+    from .expert_ops import quantize_mxfp4
+    row = pack_expert(gate_w, up_w, down_w)
+    out = torch.empty(row.numel() // 32 * 17, dtype=torch.uint8, device=row.device)
+    quantize_mxfp4(row, out=mxfp4_parts(out))
+    return out
+
+
 def read_spec(model_path):
     return spec_from_config(json.loads((Path(model_path) / 'config.json').read_text()))
 

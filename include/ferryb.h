@@ -109,6 +109,105 @@ FERRYB_API int ferryb_execute_experts_noalloc(const void* cache, int64_t cache_s
                                               ferryb_stream_t stream);
 
 /* ------------------------------------------------------------------------
+ * Routing from router logits, for routers that kernel 1 does not compute
+ * (kernel 1: softmax top-k as the hooks of ferry/model.py:137-158 have it):
+ * softmax or sigmoid scores, a balance bias on the selection, groups of
+ * consecutive experts, renormalised and scaled weights.  Its outputs are the
+ * `selected` and (bf16) `weights` of ferryb_layer_execute.
+ *
+ * score_e = softmax(logits)_e or 1 / (1 + exp(-logits_e)); key_e = score_e +
+ * bias_e.  With n_group > 1 the topk_group groups of the largest worth (their
+ * largest key, or the sum of their two largest) stay.  selected: the topk
+ * largest keys, descending; ties go to the lower id; a NaN key ranks below
+ * every number.  weights: the selected scores (no bias), divided by their sum
+ * if norm_topk (0 where the sum is 0), times scaling.  A row of -inf logits
+ * has the weights 0 with softmax.  Scores and keys are formed in 64 bits.
+ * Limits: 1024 experts, topk <= 32, n_group <= 32, at most 32 * (the power of
+ * two <= 32 / n_group) experts in a group.  Asynchronous on `stream`.
+ */
+enum { FERRYB_BF16 = 0, FERRYB_FP16 = 1, FERRYB_FP32 = 2 };
+enum { FERRYB_SOFTMAX = 0, FERRYB_SIGMOID = 1 };
+enum { FERRYB_GROUP_MAX = 0, FERRYB_GROUP_TOP2 = 1 };
+
+typedef struct ferryb_route_args {
+  const void* logits;  /* device [tokens, experts], rows row_stride elements apart */
+  int64_t tokens, row_stride;
+  int32_t experts, topk, n_group, topk_group;
+  int32_t logits_type, weights_type; /* FERRYB_BF16 / FP16 / FP32 */
+  int32_t score, group_score, norm_topk;
+  float scaling;
+  const float* bias;   /* device [experts] or NULL */
+  int64_t* selected;   /* device [tokens, topk] */
+  void* weights;       /* device [tokens, topk] of weights_type */
+} ferryb_route_args;
+FERRYB_API int ferryb_route_experts(const ferryb_route_args* args, ferryb_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * MXFP4 (OCP microscaling, e2m1 elements in blocks of 32 along a row with one
+ * power-of-two scale each; no counterpart in the reference, whose experts are
+ * bf16).  A block's scale byte s stands for 2^(s - 127): s = the exponent
+ * field of the block's largest magnitude as a float32, minus 2, at least 0.
+ * Its codes (two a byte, the lower nibble first) are the values times
+ * 2^(127 - s) rounded half to even to {0, 0.5, 1, 1.5, 2, 3, 4, 6} and their
+ * negatives, at most 6.  A block with an infinity or a NaN gets s = 255 and
+ * codes 0, and reads back as NaN.
+ *
+ * x: device [rows, width] of x_type, width a multiple of 32, rows x_stride
+ * elements apart; codes: device, width / 2 bytes a row, rows codes_stride
+ * bytes apart; scales: device, width / 32 bytes a row, rows scales_stride
+ * bytes apart (both may be parts of one buffer, such as an expert row).
+ * dequantize: y = code * 2^(s - 127), rounded once to y_type.  Asynchronous
+ * on `stream`. */
+FERRYB_API int ferryb_quantize_mxfp4(const void* x, int32_t x_type, int64_t rows, int64_t width,
+                                     int64_t x_stride, void* codes, int64_t codes_stride,
+                                     void* scales, int64_t scales_stride, ferryb_stream_t stream);
+FERRYB_API int ferryb_dequantize_mxfp4(const void* codes, int64_t codes_stride, const void* scales,
+                                       int64_t scales_stride, int64_t rows, int64_t width, void* y,
+                                       int32_t y_type, int64_t y_stride, ferryb_stream_t stream);
+
+/* Routed-expert SwiGLU over MXFP4 expert rows (tcgen05, weights expanded on
+ * the way into tensor memory): ferryb_execute_experts for 4-bit experts, with
+ * the group table on the device and no host synchronisation.
+ *
+ * cache: 16-byte aligned device bytes [cache_slots, 3 * hidden * intermediate
+ * * 17 / 32]; a row is the codes of [gate I x H | up I x H | down H x I] (see
+ * ferryb_quantize_mxfp4), then their scale bytes in the same order.  Group g
+ * is routes [starts[g], starts[g + 1]) with the weights of slots[g]; groups may
+ * be empty, and output rows of routes outside [starts[0], starts[n_groups])
+ * are left as they were.  out[p] = (silu(x Wg^T) * (x Wu^T)) Wd^T *
+ * routing_weights[rows[p], cols[p]], x = input[rows[p]], rounded to bf16 once;
+ * the activation is rounded to bf16, gate and up are not.
+ * Errors found on the device set *err (4, if it was 0) and go on: a row, column
+ * or slot out of range makes its routes' outputs NaN; with starts out of order
+ * or range no row is written.  *err = 1: a
+ * wait inside the kernel ran out, no output is valid.
+ * hidden and intermediate: multiples of 128, at most 65536.  The workspace is
+ * 256-byte aligned, not shared by calls that may overlap. */
+typedef struct ferryb_mxfp4_experts_args {
+  const void* cache;
+  int64_t cache_slots;
+  const void* input;           /* device bf16 [n_input, hidden], rows input_stride elements apart */
+  int64_t n_input, input_stride;
+  const void* routing_weights; /* device [n_input, topk] of weights_type */
+  int64_t topk;
+  int32_t weights_type, reserved;
+  const int64_t* slots;        /* device [n_groups] */
+  const int64_t* starts;       /* device [n_groups + 1] */
+  int64_t n_groups;
+  const int64_t* rows;         /* device [routes] */
+  const int64_t* cols;         /* device [routes] */
+  int64_t routes, hidden, intermediate;
+  void* out;                   /* device bf16 [routes, hidden] */
+  void* workspace;
+  int64_t workspace_bytes;
+  int32_t* err;                /* device [1] */
+} ferryb_mxfp4_experts_args;
+FERRYB_API int64_t ferryb_execute_experts_mxfp4_workspace(int64_t routes, int64_t n_groups,
+                                                          int64_t hidden, int64_t intermediate);
+FERRYB_API int ferryb_execute_experts_mxfp4(const ferryb_mxfp4_experts_args* args,
+                                            ferryb_stream_t stream);
+
+/* ------------------------------------------------------------------------
  * Kernel 2: placement planner (one CTA, bit-exact with the reference).
  * Replaces Controller.plan -> plan_layer (ferry/policy.py:130-194, :208-228)
  * with _demand (:25-33), _admission_capacity (:36-46), the quota LUT and
