@@ -1,40 +1,49 @@
 // experts_mxfp4.cu -- routed-expert SwiGLU over MXFP4 expert rows: a grouped
-// GEMM on the 5th-generation tensor cores whose weight operand is expanded from
-// 4 bits on its way into tensor memory.
+// GEMM on the 5th-generation tensor cores with block-scaled operands
+// (tcgen05.mma kind::mxf8f6f4), so that 4-bit weights go from memory into the
+// MMA without a single instruction spent on expanding them.
 //
 // The operator beside execute_experts (ferry/csrc/expert_ops.cpp:16-45): per
 // group of routes, y = (silu(x Wg^T) * (x Wu^T)) Wd^T * w with W = code *
-// 2^(scale - 127).  Every such weight is a bf16 number, so the products are the
-// exact ones of bf16 operands; sums, gate, up and silu stay in float32, and two
-// roundings to bf16 remain: the activation (it is the second product's tensor-
-// core operand) and the result.
+// 2^(scale - 127).
 //
-// Data layout.  A cache row is [gate I x H | up I x H | down H x I] codes, two
-// a byte, then their scale bytes in the same order, one for 32 codes.  Groups
-// of more than 128 routes are split into sub-groups of nearly equal size, each
-// with its own work items, so that a popular expert is spread over the GPU.
+// Operands.  A = weights: e2m1 codes, one scale byte for 32 columns, exactly as
+// they lie in the cache row ([gate I x H | up I x H | down H x I] codes, two a
+// byte, then their scale bytes in the same order).  B = routes: a bf16 number
+// has 8 significant bits and an e4m3 number 4, so a row is stored as two e4m3
+// parts, hi (the value rounded to e4m3) and lo (what is left of it), each with
+// a power-of-two scale for 32 columns, the lo scale 2^-4 of the hi one; both
+// parts are multiplied and summed into the same float32 accumulator.  A block's
+// largest value is brought to [2^7, 2^8); hi + lo is then the bf16 number itself
+// down to 2^-6 (2^-13 of the largest) and within 2^-14 (2^-21 of the largest)
+// below that, half the lo part's smallest step of 2^-9 * 2^-4.  The activation,
+// operand of the second product, is stored the same way: hi + lo rounds it to
+// within 2^-9 of its value (bf16: 2^-9), or 2^-21 of its block's largest.  Gate, up and silu stay in float32, the result is rounded
+// to bf16 once.
 //
 // Orientation as in experts.cu: 128 weight rows are the MMA's M side (64 gate
 // rows above the 64 up rows of the same features, or 128 down rows), the routes
-// its N side.  The weight operand comes from tensor memory (tcgen05.mma takes A
-// from there): a thread expands one row's codes in registers and stores them
-// with tcgen05.st, so expanded weights touch neither shared memory nor a
-// swizzle, and shared memory carries codes and routes only.
+// its N side.  Groups are split into sub-groups of at most 32, 64 or 128 routes
+// (by the mean of the groups: small groups need no wide tiles, and narrow ones
+// leave shared memory to the weights), each with its own work items, so that a
+// popular expert is spread over the GPU.
 //
-// Expansion.  Of a 32-bit word of 8 codes, shifts and masks put code j into the
-// sign, the two low exponent bits and the top mantissa bit of a bf16, and code
-// j + 4 into the upper half: as a bf16 that pattern is the e2m1 value times
-// 2^-126 (subnormals included), and one bf16x2 multiply by 2^(scale - 1) makes
-// both weights exactly.  The order (0 4 1 5 2 6 3 7) of every 8 columns is met
-// by storing the routes' columns in the same order.
+// Data flow of a step (128 columns): TMA unpacks the codes of 128 weight rows
+// into 16 KB of shared memory (4-bit data in 8-bit places, 128-byte swizzle, as
+// the MMA reads them) and brings the routes' hi and lo parts; cp.async brings
+// the weight rows' 4 scale bytes each (pieces of 4 bytes need no padding of the
+// scale rows); four warps move the scales of both sides into tensor memory
+// (row r in lane r % 32 of every 32-lane quarter, column r / 32, one byte for
+// each 32 columns of the step); one thread issues the 8 MMAs of K = 32, hi and
+// lo for each scale byte.
 //
-// CTA roles (480 threads): warp 0 claims work and loads codes (TMA) and scales
-// (cp.async, whose 4-byte pieces need no padding of the scale rows); warp 14
-// loads the routes (TMA); warps 6-13 expand, four on even and four on odd
-// k-steps (warp w owns TMEM lanes 32 * (w % 4)..+31); warp 1 issues the MMAs;
-// warps 2-5 drain the accumulators.  Codes do not depend on phase 1, so warp 0
-// runs ahead into phase 2 while warp 14 waits for the activations.
+// CTA roles (480 threads): warp 0 claims work and loads codes and scales; warp
+// 1 issues the MMAs; warps 2-5 and 6-9 drain the two accumulators; warp 10
+// loads the routes; warps 11-14 move the scales.  Codes do not depend on phase
+// 1, so warp 0 runs ahead into phase 2 while the routes' warps wait for the
+// activations.
 #include <cuda_fp16.h>
+#include <cuda_fp8.h>
 
 #include <atomic>
 
@@ -44,23 +53,23 @@
 namespace ferryb {
 
 constexpr int kMxWarps = 15;
-constexpr int kMxThreadsG = kMxWarps * 32;
+constexpr int kMxThreads = kMxWarps * 32;
+constexpr int kFirstEpi = 2, kRouteWarp = 10, kFirstScale = 11;
 constexpr int kMxM = 128;          // weight rows per tile
-constexpr int kMxN = 128;          // routes per sub-group
-constexpr int kMxStepK = 64;       // columns per MMA step (one swizzled 128-byte row of routes)
-constexpr int kMxChunkK = 256;     // columns per code stage (128 bytes of codes a row)
+constexpr int kMxN = 128;          // most routes of a sub-group
+constexpr int kStepK = 128;        // columns per step
 constexpr int kMxFeatures = 64;    // gate (= up) rows per phase-1 tile
-constexpr int kCodeStages = 4;
-constexpr int kSteps = 8;          // route stages = expanded-weight stages
-constexpr uint32_t kCodeBytes = kMxM * 128;
-constexpr uint32_t kScaleBytes = kMxM * 8;
-constexpr uint32_t kRouteBytes = kMxN * kMxStepK * 2;
-constexpr uint32_t kTmemW = 256;   // first TMEM column of the expanded weights
+constexpr int kBars = 16;          // barriers of the step pipeline, more than any buffer's depth
+constexpr int kScaleStages = 8;    // steps whose scales tensor memory holds
+constexpr uint32_t kCodeBytes = kMxM * kStepK;  // unpacked
+constexpr uint32_t kScaleBytes = kMxM * 4;
+constexpr uint32_t kTmemScale = 256;  // first TMEM column of the scales, 16 a step
 constexpr int kRing = 4;           // claimed items in flight
 constexpr int kXStride = 17;       // floats a feature of the gate/up exchange (padded)
-constexpr uint32_t kXchgBytes = 2 * kMxFeatures * kXStride * 4;
-constexpr uint32_t kMxSmem = kCodeStages * (kCodeBytes + kScaleBytes) + kSteps * kRouteBytes +
-                             kXchgBytes + 512 + 1024;
+constexpr uint32_t kXchgBytes = 2 * kMxFeatures * kXStride * 4;  // an epilogue group's
+constexpr uint32_t kPoolBytes = 12 * 16384;  // codes and routes
+constexpr int kMaxCodeStages = 10;
+constexpr uint32_t kMxSmem = kPoolBytes + kMaxCodeStages * kScaleBytes + 1024 + 1024;
 constexpr uint64_t kMxWaitNs = 2000000000ull;  // bound on any wait
 
 // Up to 128 routes of one group.
@@ -71,54 +80,95 @@ struct MxGroup {
   int32_t bad;    // slot out of range: the routes' outputs are NaN
 };
 
+// Written by the prepare kernel.
+struct MxHeader {
+  int queue;     // claim counter
+  int n_groups;  // sub-groups
+  int box;       // 0..3: sub-groups of at most 16, 32, 64, 128 routes
+};
+
 struct MxParams {
   const MxGroup* groups;
-  const int* n_groups;  // [1] sub-groups, written by the prepare kernel
+  MxHeader* header;
   int mt1, mt2;         // items per sub-group: I / 64 phase 1, H / 128 phase 2
   int hidden, inter;
   const uint8_t* scales;  // slot 0's scale bytes
   int64_t row_bytes;      // bytes of a cache row
-  __nv_bfloat16* act;
+  const uint8_t* xs;      // hi scale bytes of the routes [routes, pitch1]
+  uint8_t* act;           // [routes, 2 * I]: hi, lo
+  uint8_t* as;            // hi scale bytes of the activations [routes, pitch2]
+  int pitch1, pitch2;
   __nv_bfloat16* out;
   const float* route_w;
-  int* queue;  // [1] claim counter, zero at launch
   int* dep;    // [sub-groups] phase-1 epilogue-warp completions, zero at launch
   int* err;
 };
 
+struct MxMaps {
+  CUtensorMap w1, w2;        // codes of gate and up rows (64-row boxes), of down rows (128)
+  CUtensorMap x16, x64;      // routes [routes, 2 * H], boxes of 16 and 64 rows
+  CUtensorMap a16, a64;      // activations [routes, 2 * I]
+};
+
+// A claimed work item, handed from warp 0 to the other roles.
 struct MxItem {
-  int phase, group, tile;
+  int phase;  // 1, 2 or 0 = no more work
+  int group, tile;
+  int start, count, bad;  // of the sub-group
+  int slot, pad;
 };
 
 __device__ __forceinline__ MxItem mx_item(const MxParams& p, int n_groups, int item) {
-  MxItem it;
+  MxItem it{};
   const int n1 = n_groups * p.mt1;
   if (item < n1) {
     it.phase = 1; it.group = item / p.mt1; it.tile = item - it.group * p.mt1;
-  } else {
+  } else if (item < n1 + n_groups * p.mt2) {
     const int i = item - n1;
     it.phase = 2; it.group = i / p.mt2; it.tile = i - it.group * p.mt2;
+  } else {
+    return it;
   }
+  const MxGroup g = p.groups[it.group];
+  it.start = g.start; it.count = g.count; it.bad = g.bad; it.slot = g.slot;
   return it;
 }
 
+// One wait of at most about 20 us: the hint lets the hardware suspend the warp,
+// which otherwise polls and takes issue slots from the warps that expand.
+__device__ __forceinline__ bool mx_try_wait(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(20000u)
+      : "memory");
+  return ok != 0;
+}
 // Wait for an mbarrier phase, bounded in time; on time-out the CTA's abort flag
-// and the error word are set.
-__device__ __forceinline__ bool mx_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
-                                        int* err) {
-  if (mbar_try_wait(bar, parity)) return true;
+// and the error word are set.  The clock is read only once a wait has become
+// long.
+__device__ __noinline__ bool mx_wait_long(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
+                                          int* err) {
   const uint64_t t0 = globaltimer_ns();
-  for (uint32_t i = 1;; ++i) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if ((i & 255) == 0) {
-      if (*abort_flag) return false;
-      if (globaltimer_ns() - t0 > kMxWaitNs) {
-        *abort_flag = 1;
-        atomicCAS(err, 0, DEV_WAIT_TIMEOUT);
-        return false;
-      }
+  for (;;) {
+    for (int i = 0; i < 16; ++i)
+      if (mx_try_wait(bar, parity)) return true;
+    if (*abort_flag) return false;
+    if (globaltimer_ns() - t0 > kMxWaitNs) {
+      *abort_flag = 1;
+      atomicCAS(err, 0, DEV_WAIT_TIMEOUT);
+      return false;
     }
   }
+}
+__device__ __forceinline__ bool mx_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
+                                        int* err) {
+  for (int i = 0; i < 8; ++i)
+    if (mx_try_wait(bar, parity)) return true;
+  return mx_wait_long(bar, parity, abort_flag, err);
 }
 // The same for a whole warp: all lanes agree on the outcome.
 __device__ __forceinline__ bool mx_wait_warp(uint64_t* bar, uint32_t parity,
@@ -143,120 +193,139 @@ __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
-// 32 lanes x 32 columns of 32 bits into tensor memory.
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
-      "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
-      "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-      : "memory");
+// 32 lanes x 4 columns of 32 bits into tensor memory.
+__device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
-// D[tmem] (+)= A[tmem] x B[smem]^T, bf16 inputs, float32 accumulate.
-__device__ __forceinline__ void umma_bf16_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc,
-                                             uint32_t idesc, uint32_t accumulate) {
+// D[tmem] (+)= (A[smem] * scales) x (B[smem] * scales)^T, 32 columns: e2m1 codes
+// in 8-bit places times e4m3, float32 accumulate, one UE8M0 scale for the 32.
+__device__ __forceinline__ void umma_mxf8f6f4(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc,
+                                              uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                              uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
-      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], "
+      "p;\n\t}" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
       : "memory");
 }
-
-__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
-  uint32_t d;
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-  return d;
+// Instruction descriptor of kind::mxf8f6f4: A e2m1 (5 in bits 7-9), B e4m3 (0 in
+// bits 10-12), both K-major, N >> 3 in bits 17-22, UE8M0 scales (bit 23), M >> 7
+// in bits 27-28; the scale byte a K-block takes from its 32-bit columns is in
+// bits 4-5 for B and 29-30 for A.
+__device__ __forceinline__ uint32_t mx_idesc(uint32_t n, uint32_t byte) {
+  return (5u << 7) | ((n >> 3) << 17) | (1u << 23) | (1u << 27) | (byte << 4) | (byte << 29);
 }
 
-// 8 codes of a word -> 4 x bf16x2 (codes j and j + 4) times 2^-126.
-__device__ __forceinline__ void spread8(uint32_t w, uint32_t* o) {
-  constexpr uint32_t kMag = 0x01C001C0u, kSign = 0x80008000u;
-  o[0] = ((w << 6) & kMag) | ((w << 12) & kSign);
-  o[1] = ((w << 2) & kMag) | ((w << 8) & kSign);
-  o[2] = ((w >> 2) & kMag) | ((w << 4) & kSign);
-  o[3] = ((w >> 6) & kMag) | (w & kSign);
+// ---- hi and lo parts of values ----
+// Scale byte of a block whose largest magnitude has the float32 exponent field
+// `field`: the block's values times 2^(127 - byte) stay below 2^8.  At least 4,
+// so that the lo scale (byte - 4) exists; 255 (NaN) if a value is not finite.
+__device__ __forceinline__ int mx_block_byte(uint32_t field) {
+  return field == 255u ? 255 : max(static_cast<int>(field) - 7, 4);
+}
+__device__ __forceinline__ float mx_block_mult(int byte) {
+  return byte == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float(static_cast<uint32_t>(254 - byte) << 23);
+}
+// Two values (already times 2^(127 - byte)) -> two hi bytes and two lo bytes.
+__device__ __forceinline__ void mx_split2(float a, float b, uint32_t* hi, uint32_t* lo) {
+  const __nv_fp8x2_storage_t h = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  const float2 back = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(h, __NV_E4M3)));
+  const __nv_fp8x2_storage_t l = __nv_cvt_float2_to_fp8x2(
+      make_float2((a - back.x) * 16.0f, (b - back.y) * 16.0f), __NV_SATFINITE, __NV_E4M3);
+  *hi = h;
+  *lo = l;
 }
 
-// 32 codes and their scale byte -> 16 x bf16x2.  2^(s - 127) * 2^126 is a bf16
-// up to s = 128 (blocks whose largest value is below 16); beyond, the factor is
-// applied in two steps.  s = 255 stands for NaN.
-__device__ __forceinline__ void expand32(const uint4& c, uint32_t s, uint32_t* o) {
-  const uint32_t m = min(s + 126u, 254u) * 0x00800080u;
-  spread8(c.x, o);
-  spread8(c.y, o + 4);
-  spread8(c.z, o + 8);
-  spread8(c.w, o + 12);
-#pragma unroll
-  for (int i = 0; i < 16; ++i) o[i] = mul_bf16x2(o[i], m);
-  if (s > 128u) {
-    const uint32_t m2 = s == 255u ? 0x7FC07FC0u : (s - 1u) * 0x00800080u;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) o[i] = mul_bf16x2(o[i], m2);
-  }
+// The four warps of epilogue group g (0 or 1) meet at named barrier 1 + g, and
+// leave their loop together: every decision goes through a barrier that ANDs
+// it.
+__device__ __forceinline__ void mx_epilogue_sync(int g) {
+  asm volatile("bar.sync %0, 128;" ::"r"(1 + g) : "memory");
 }
-
-__device__ __forceinline__ void mx_epilogue_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
-// The four epilogue warps leave their loop together: every decision goes
-// through a barrier that ANDs it.
-__device__ __forceinline__ bool mx_epilogue_all(bool v) {
+__device__ __forceinline__ bool mx_epilogue_all(int g, bool v) {
   uint32_t r;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.u32 p, %1, 0;\n\t"
-      "bar.red.and.pred q, 1, 128, p;\n\t"
+      "bar.red.and.pred q, %2, 128, p;\n\t"
       "selp.u32 %0, 1, 0, q;\n\t}"
       : "=r"(r)
-      : "r"(static_cast<uint32_t>(v))
+      : "r"(static_cast<uint32_t>(v)), "r"(1 + g)
       : "memory");
   return r != 0;
 }
 
-__device__ __forceinline__ int mx_box(int n) { return n <= 16 ? 0 : n <= 32 ? 1 : n <= 64 ? 2 : 3; }
+// The pool of shared memory, by the sub-groups' size: stages of codes first,
+// then stages of routes (hi and lo parts of `box` rows).  Deep code rings where
+// routes are few (memory-bound), enough of both where they are many.
+__host__ __device__ __forceinline__ int mx_code_stages(int box) {
+  return box == 0 ? 10 : box == 1 ? 9 : box == 2 ? 8 : 4;
+}
+__host__ __device__ __forceinline__ int mx_route_stages(int box) {
+  return box == 0 ? 8 : box == 1 ? 6 : 4;
+}
+__host__ __device__ __forceinline__ uint32_t mx_route_bytes(int box) { return (16u << box) * kStepK * 2; }
 
-// Column of feature f in the stored order of every 8 columns.
-__device__ __forceinline__ int mx_column(int f) {
-  const int e = f & 7;
-  return (f & ~7) | (e < 4 ? 2 * e : 2 * e - 7);
+// Steps are numbered from 0 over all items of a CTA.  Step t uses barrier t % 16
+// of each pipeline; a buffer of S stages may be refilled for step t once step
+// t - S is done, and S < 16 keeps the parity unambiguous.
+__device__ __forceinline__ bool mx_wait_step(uint64_t* bars, uint32_t t, volatile int* abort_flag,
+                                             int* err) {
+  return mx_wait(bars + t % kBars, (t / kBars) & 1, abort_flag, err);
 }
 
-__global__ void __launch_bounds__(kMxThreadsG, 1)
-    mxfp4_swiglu_kernel(const __grid_constant__ CUtensorMap w1, const __grid_constant__ CUtensorMap w2,
-                        const __grid_constant__ BMaps bx, const __grid_constant__ BMaps ba,
-                        const MxParams p) {
+// Wait until the sub-group's activations are written: four epilogue warps for
+// each of its phase-1 tiles.
+__device__ __forceinline__ bool mx_wait_dep(const int* dep, uint32_t want, volatile int* abort_flag,
+                                            int* err) {
+  const uint32_t* cnt = reinterpret_cast<const uint32_t*>(dep);
+  if (ld_acquire_gpu_u32(cnt) >= want) return true;
+  const uint64_t t0 = globaltimer_ns();
+  while (ld_acquire_gpu_u32(cnt) < want) {
+    __nanosleep(32);
+    if (*abort_flag) return false;
+    if (globaltimer_ns() - t0 > kMxWaitNs) {
+      *abort_flag = 1;
+      atomicCAS(err, 0, DEV_WAIT_TIMEOUT);
+      return false;
+    }
+  }
+  return true;
+}
+
+__global__ void __launch_bounds__(kMxThreads, 1)
+    mxfp4_swiglu_kernel(const __grid_constant__ MxMaps maps, const MxParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
-  uint8_t* codes = smem;
-  uint8_t* routes = codes + kCodeStages * kCodeBytes;
-  uint8_t* scale = routes + kSteps * kRouteBytes;
-  float* xchg = reinterpret_cast<float*>(scale + kCodeStages * kScaleBytes);
-  uint64_t* cfull = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(xchg) + kXchgBytes);
-  uint64_t* cempty = cfull + kCodeStages;
-  uint64_t* rfull = cempty + kCodeStages;  // routes landed
-  uint64_t* wfull = rfull + kSteps;        // weights expanded
-  uint64_t* sempty = wfull + kSteps;       // step consumed by the MMA
-  uint64_t* tfull = sempty + kSteps;       // [2] accumulators
+  uint8_t* scale = smem + kPoolBytes;  // [code stages][128 rows] 4 scale bytes
+  uint64_t* full = reinterpret_cast<uint64_t*>(scale + kMaxCodeStages * kScaleBytes);
+  uint64_t* kfull = full + kBars;    // the weights' scale bytes landed
+  uint64_t* done = kfull + kBars;    // the MMAs of a step are complete
+  uint64_t* tfull = done + kBars;    // [2] accumulators
   uint64_t* tempty = tfull + 2;
-  uint64_t* ifull = tempty + 2;            // [kRing] claimed items
+  uint64_t* ifull = tempty + 2;      // [kRing] claimed items
   uint64_t* iempty = ifull + kRing;
   uint64_t* drain = iempty + kRing;
-  int* ring = reinterpret_cast<int*>(drain + 1);
-  uint32_t* tmem_smem = reinterpret_cast<uint32_t*>(ring + kRing);
+  uint32_t* tmem_smem = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_smem + 1);
+  MxItem* ring = reinterpret_cast<MxItem*>(drain + 2);  // [kRing]
+  __shared__ float xchg_all[2][kXchgBytes / 4];
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kCodeStages; ++s) { mbar_init(&cfull[s], 33); mbar_init(&cempty[s], 8); }
-    for (int s = 0; s < kSteps; ++s) {
-      mbar_init(&rfull[s], 1);
-      mbar_init(&wfull[s], 4);
-      mbar_init(&sempty[s], 1);
+    for (int s = 0; s < kBars; ++s) {
+      mbar_init(&full[s], 6);    // codes, routes and four scale warps
+      mbar_init(&kfull[s], 32);  // cp.async of warp 0's lanes
+      mbar_init(&done[s], 1);
     }
     for (int b = 0; b < 2; ++b) { mbar_init(&tfull[b], 1); mbar_init(&tempty[b], 4); }
     for (int q = 0; q < kRing; ++q) { mbar_init(&ifull[q], 1); mbar_init(&iempty[q], 14); }
@@ -269,166 +338,219 @@ __global__ void __launch_bounds__(kMxThreadsG, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_smem;
-  const int n_groups = *p.n_groups;
-  const int n_items = n_groups * (p.mt1 + p.mt2);
+  const int box = p.header->box;
+  const uint32_t code_stages = mx_code_stages(box), route_stages = mx_route_stages(box);
+  const uint32_t route_bytes = mx_route_bytes(box);
+  uint8_t* const routes = smem + code_stages * kCodeBytes;
   int q = 0;            // this role's place in the item ring
   uint32_t qphase = 0;
 
   if (warp == 0) {
     // ---------------- claims, codes and scales ----------------
-    int stage = 0;
-    uint32_t phase = 0, pending = 0, pend_parity = 0;
+    uint32_t t = 0, stage = 0;
     bool ok = true;
+    const int n_groups = p.header->n_groups;
+    int next = lane == 0 ? atomicAdd(&p.header->queue, 1) : 0;
     while (ok) {
+      const MxItem it = mx_item(p, n_groups, __shfl_sync(0xffffffffu, next, 0));
       if (!mx_wait_warp(&iempty[q], qphase ^ 1, abort_flag, p.err)) { ok = false; break; }
-      int item = 0;
       if (lane == 0) {
-        item = atomicAdd(p.queue, 1);
-        if (item >= n_items || *abort_flag) item = -1;
-        ring[q] = item;
+        ring[q] = it;
         mbar_arrive(&ifull[q]);
       }
-      item = __shfl_sync(0xffffffffu, item, 0);
       if (++q == kRing) { q = 0; qphase ^= 1; }
-      if (item < 0) break;
-      const MxItem it = mx_item(p, n_groups, item);
-      const MxGroup g = p.groups[it.group];
+      if (it.phase == 0) break;
+      if (lane == 0) next = atomicAdd(&p.header->queue, 1);  // back before this item's loads are issued
       const int K = it.phase == 1 ? p.hidden : p.inter;
-      // first scale byte of the rows this lane copies: tile rows lane + 32 * i
-      const uint8_t* src = p.scales + static_cast<int64_t>(g.slot) * p.row_bytes;
-      const int64_t pitch = K / 32;
-      int64_t row0;  // matrix row of tile row 0
-      if (it.phase == 1) {
-        row0 = static_cast<int64_t>(it.tile) * kMxFeatures;
-      } else {
-        src += 2 * static_cast<int64_t>(p.inter) * (p.hidden / 32);
-        row0 = static_cast<int64_t>(it.tile) * kMxM;
-      }
-      for (int k0 = 0; k0 < K; k0 += kMxChunkK) {
-        if (!mx_wait_warp(&cempty[stage], phase ^ 1, abort_flag, p.err)) { ok = false; break; }
-        uint8_t* cs = codes + stage * kCodeBytes;
+      // scale bytes of the tile rows that this lane copies: lane + 32 * i
+      const int pitch = K / 32;
+      const int row0 = it.tile * (it.phase == 1 ? kMxFeatures : kMxM);
+      const uint8_t* src = p.scales + it.slot * p.row_bytes + static_cast<int64_t>(row0 + lane) * pitch +
+                           (it.phase == 1 ? 0 : 2 * static_cast<int64_t>(p.inter) * (p.hidden / 32));
+      const int64_t d1 = 32 * pitch;
+      const int64_t d2 = it.phase == 1 ? static_cast<int64_t>(p.inter) * pitch : 2 * d1;  // up rows
+      for (int k0 = 0; k0 < K; k0 += kStepK, ++t) {
+        if (t >= code_stages &&
+            !__all_sync(0xffffffffu, mx_wait_step(done, t - code_stages, abort_flag, p.err))) {
+          ok = false;
+          break;
+        }
         if (lane == 0) {
-          mbar_expect_tx(&cfull[stage], kCodeBytes);
+          uint64_t* bar = full + t % kBars;
+          uint8_t* cs = smem + stage * kCodeBytes;
+          mbar_expect_tx(bar, kCodeBytes / 2);  // the copy counts its 4-bit data, not the gaps
           if (it.phase == 1) {
-            tma_load_3d(cs, &w1, &cfull[stage], k0 / 2, static_cast<int>(row0), g.slot);
-            tma_load_3d(cs + kCodeBytes / 2, &w1, &cfull[stage], k0 / 2, p.inter + static_cast<int>(row0),
-                        g.slot);
+            tma_load_3d(cs, &maps.w1, bar, k0, row0, it.slot);
+            tma_load_3d(cs + kCodeBytes / 2, &maps.w1, bar, k0, p.inter + row0, it.slot);
           } else {
-            tma_load_3d(cs, &w2, &cfull[stage], k0 / 2, static_cast<int>(row0), g.slot);
+            tma_load_3d(cs, &maps.w2, bar, k0, row0, it.slot);
           }
         }
-        uint8_t* ss = scale + stage * kScaleBytes;
-        const bool whole = K - k0 >= kMxChunkK;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = lane + 32 * i;
-          const int64_t row = it.phase == 1 && r >= kMxFeatures ? p.inter + row0 + r - kMxFeatures
-                                                                : row0 + r;
-          const uint8_t* from = src + row * pitch + k0 / 32;
-          cp_async4(ss + r * 8, from);
-          if (whole) cp_async4(ss + r * 8 + 4, from + 4);
-        }
-        cp_async_arrive(&cfull[stage]);
-        pending |= 1u << stage;
-        pend_parity = (pend_parity & ~(1u << stage)) | (phase << stage);
-        if (++stage == kCodeStages) { stage = 0; phase ^= 1; }
+        uint8_t* ss = scale + stage * kScaleBytes + lane * 4;
+        cp_async4(ss, src);
+        cp_async4(ss + 128, src + d1);
+        cp_async4(ss + 256, src + d2);
+        cp_async4(ss + 384, src + d2 + d1);
+        cp_async_arrive(&kfull[t % kBars]);
+        src += kStepK / 32;
+        if (++stage == code_stages) stage = 0;
       }
     }
     if (!ok) {
-      // the other roles stop at the abort flag; let this CTA's loads land first
+      // the other roles stop at the abort flag; this CTA's loads get a bounded
+      // time to land (a step's barrier may lack another role's arrival now)
       *abort_flag = 1;
       asm volatile("cp.async.wait_all;" ::: "memory");
       const uint64_t t0 = globaltimer_ns();
-      for (int s = 0; s < kCodeStages; ++s)
-        if (pending & (1u << s))
-          while (!mbar_try_wait(&cfull[s], (pend_parity >> s) & 1) && globaltimer_ns() - t0 < kMxWaitNs) {}
+      while (globaltimer_ns() - t0 < 1000000) {}
     }
-  } else if (warp == 14) {
+  } else if (warp == kRouteWarp) {
     // ---------------- routes ----------------
-    int stage = 0;
-    uint32_t phase = 0, pending = 0, pend_parity = 0;
-    bool ok = true;
     if (elect_one()) {
+      uint32_t t = 0, stage = 0;
+      bool ok = true;
       while (ok) {
         if (!mx_wait(&ifull[q], qphase, abort_flag, p.err)) { ok = false; break; }
-        const int item = ring[q];
+        const MxItem it = ring[q];
         mbar_arrive(&iempty[q]);
         if (++q == kRing) { q = 0; qphase ^= 1; }
-        if (item < 0) break;
-        const MxItem it = mx_item(p, n_groups, item);
-        const MxGroup g = p.groups[it.group];
+        if (it.phase == 0) break;
         if (it.phase == 2) {
-          // the sub-group's activations: four epilogue warps for each phase-1 tile
-          const uint32_t want = 4 * p.mt1;
-          const uint32_t* cnt = reinterpret_cast<const uint32_t*>(p.dep + it.group);
-          const uint64_t t0 = globaltimer_ns();
-          while (ld_acquire_gpu_u32(cnt) < want) {
-            __nanosleep(64);
-            if (*abort_flag) { ok = false; break; }
-            if (globaltimer_ns() - t0 > kMxWaitNs) {
-              *abort_flag = 1;
-              atomicCAS(p.err, 0, DEV_WAIT_TIMEOUT);
-              ok = false;
-              break;
-            }
-          }
-          if (!ok) break;
+          if (!mx_wait_dep(p.dep + it.group, 4 * p.mt1, abort_flag, p.err)) { ok = false; break; }
           asm volatile("fence.proxy.async.global;" ::: "memory");
         }
-        const BMaps* bm = it.phase == 1 ? &bx : &ba;
-        const int bi = mx_box(g.count);
-        const uint32_t bytes = (16u << bi) * kMxStepK * 2;
-        const int steps = (it.phase == 1 ? p.hidden : p.inter) / kMxStepK;
-        for (int kb = 0; kb < steps; ++kb) {
-          if (!mx_wait(&sempty[stage], phase ^ 1, abort_flag, p.err)) { ok = false; break; }
-          mbar_expect_tx(&rfull[stage], bytes);
-          tma_load_2d(routes + stage * kRouteBytes, &bm->m[bi], &rfull[stage], kb * kMxStepK, g.start);
-          pending |= 1u << stage;
-          pend_parity = (pend_parity & ~(1u << stage)) | (phase << stage);
-          if (++stage == kSteps) { stage = 0; phase ^= 1; }
+        const int K = it.phase == 1 ? p.hidden : p.inter;
+        // 16 or 32 rows in boxes of 16, 64 or 128 in boxes of 64
+        const int n = (it.count + 15) & ~15;
+        const int rows = n <= 32 ? 16 : 64;
+        const int boxes = n <= 32 ? n / 16 : (n + 63) / 64;
+        const CUtensorMap* map = it.phase == 1 ? (rows == 16 ? &maps.x16 : &maps.x64)
+                                               : (rows == 16 ? &maps.a16 : &maps.a64);
+        for (int k0 = 0; k0 < K; k0 += kStepK, ++t) {
+          if (t >= route_stages && !mx_wait_step(done, t - route_stages, abort_flag, p.err)) {
+            ok = false;
+            break;
+          }
+          uint64_t* bar = full + t % kBars;
+          uint8_t* to = routes + stage * route_bytes;
+          mbar_expect_tx(bar, static_cast<uint32_t>(boxes * rows * kStepK * 2));
+          for (int i = 0; i < boxes; ++i) {
+            tma_load_2d(to + i * rows * kStepK, map, bar, k0, it.start + i * rows);
+            tma_load_2d(to + route_bytes / 2 + i * rows * kStepK, map, bar, K + k0, it.start + i * rows);
+          }
+          if (++stage == route_stages) stage = 0;
         }
       }
       if (!ok) {
         *abort_flag = 1;
         const uint64_t t0 = globaltimer_ns();
-        for (int s = 0; s < kSteps; ++s)
-          if (pending & (1u << s))
-            while (!mbar_try_wait(&rfull[s], (pend_parity >> s) & 1) && globaltimer_ns() - t0 < kMxWaitNs) {}
+        while (globaltimer_ns() - t0 < 1000000) {}
+      }
+    }
+  } else if (warp >= kFirstScale) {
+    // ---------------- scales into tensor memory ----------------
+    // every warp writes the whole set into its own 32-lane quarter
+    const uint32_t mine = tmem + kTmemScale + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    uint32_t t = 0, stage = 0;
+    bool ok = true;
+    while (ok) {
+      if (!mx_wait_warp(&ifull[q], qphase, abort_flag, p.err)) break;
+      const int phase = ring[q].phase, group = ring[q].group, start = ring[q].start, count = ring[q].count;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&iempty[q]);
+      if (++q == kRing) { q = 0; qphase ^= 1; }
+      if (phase == 0) break;
+      if (phase == 2) {
+        bool there = true;
+        if (lane == 0) there = mx_wait_dep(p.dep + group, 4 * p.mt1, abort_flag, p.err);
+        if (!__shfl_sync(0xffffffffu, there, 0)) break;
+        __syncwarp();  // lane 0's acquire covers the warp's reads
+      }
+      const int K = phase == 1 ? p.hidden : p.inter;
+      const int pitch = phase == 1 ? p.pitch1 : p.pitch2;
+      const uint8_t* from = (phase == 1 ? p.xs : p.as) + static_cast<int64_t>(start + lane) * pitch;
+      // the routes' bytes of four steps at a time, fetched one such block ahead
+      uint4 cur[4], nxt[4];
+      auto fetch = [&](int k0, uint4* v) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          v[c] = make_uint4(0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu);
+          if (lane + 32 * c < count)
+            v[c] = __ldcg(reinterpret_cast<const uint4*>(from + static_cast<int64_t>(32 * c) * pitch + k0 / 32));
+        }
+      };
+      fetch(0, nxt);
+      for (int k0 = 0; k0 < K && ok; k0 += 4 * kStepK) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) cur[c] = nxt[c];
+        if (k0 + 4 * kStepK < K) fetch(k0 + 4 * kStepK, nxt);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (k0 + i * kStepK >= K) break;
+          uint32_t hi[4], lo[4], a[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            hi[c] = i == 0 ? cur[c].x : i == 1 ? cur[c].y : i == 2 ? cur[c].z : cur[c].w;
+            lo[c] = hi[c] - 0x04040404u;  // every byte is at least 4
+          }
+          if ((t >= kScaleStages &&
+               !__all_sync(0xffffffffu, mx_wait_step(done, t - kScaleStages, abort_flag, p.err))) ||
+              !__all_sync(0xffffffffu, mx_wait_step(kfull, t, abort_flag, p.err))) {
+            ok = false;
+            break;
+          }
+          const uint32_t* sa = reinterpret_cast<const uint32_t*>(scale + stage * kScaleBytes) + lane;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) a[c] = sa[32 * c];
+          const uint32_t at = mine + (t % kScaleStages) * 16;
+          tc_fence_after();
+          tmem_st4(at, a);
+          tmem_st4(at + 4, hi);
+          tmem_st4(at + 8, lo);
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&full[t % kBars]);
+          ++t;
+          if (++stage == code_stages) stage = 0;
+        }
       }
     }
   } else if (warp == 1) {
     // ---------------- MMA ----------------
     if (elect_one()) {
-      int stage = 0, acc = 0;
-      uint32_t phase = 0, acc_phase = 0;
+      uint32_t t = 0, cstage = 0, rstage = 0;
+      int acc = 0;
+      uint32_t acc_phase = 0;
       bool ok = true;
       while (ok) {
         if (!mx_wait(&ifull[q], qphase, abort_flag, p.err)) break;
-        const int item = ring[q];
+        const int kind = ring[q].phase;
+        const uint32_t n = static_cast<uint32_t>(ring[q].count + 15) & ~15u;
         mbar_arrive(&iempty[q]);
         if (++q == kRing) { q = 0; qphase ^= 1; }
-        if (item < 0) break;
-        const MxItem it = mx_item(p, n_groups, item);
-        const uint32_t n = static_cast<uint32_t>(p.groups[it.group].count + 15) & ~15u;
-        const uint32_t idesc = idesc_bf16_f32(kMxM, n);
-        const int steps = (it.phase == 1 ? p.hidden : p.inter) / kMxStepK;
+        if (kind == 0) break;
+        const uint32_t idesc = mx_idesc(n, 0);
+        const int steps = (kind == 1 ? p.hidden : p.inter) / kStepK;
         if (!mx_wait(&tempty[acc], acc_phase ^ 1, abort_flag, p.err)) break;
         tc_fence_after();
         const uint32_t d = tmem + acc * kMxN;
-        for (int kb = 0; kb < steps; ++kb) {
-          if (!mx_wait(&rfull[stage], phase, abort_flag, p.err) ||
-              !mx_wait(&wfull[stage], phase, abort_flag, p.err)) {
-            ok = false;
-            break;
-          }
+        for (int kb = 0; kb < steps; ++kb, ++t) {
+          if (!mx_wait_step(full, t, abort_flag, p.err)) { ok = false; break; }
           tc_fence_after();
-          const uint32_t b = smem_u32(routes + stage * kRouteBytes);
-          const uint32_t a = tmem + kTmemW + stage * 32;
+          const uint32_t a = smem_u32(smem + cstage * kCodeBytes);
+          const uint32_t b = smem_u32(routes + rstage * route_bytes);
+          const uint32_t sf = tmem + kTmemScale + (t % kScaleStages) * 16;
 #pragma unroll
-          for (int k = 0; k < kMxStepK / 16; ++k)
-            umma_bf16_ta(d, a + k * 8, smem_desc_sw128(b + k * 32), idesc, (kb > 0 || k > 0) ? 1u : 0u);
-          umma_commit(&sempty[stage]);
-          if (++stage == kSteps) { stage = 0; phase ^= 1; }
+          for (uint32_t k = 0; k < 4; ++k) {
+            const uint32_t id = idesc | (k << 4) | (k << 29);
+            const uint64_t ad = smem_desc_sw128(a + k * 32);
+            umma_mxf8f6f4(d, ad, smem_desc_sw128(b + k * 32), id, sf, sf + 4, (kb > 0 || k > 0) ? 1u : 0u);
+            umma_mxf8f6f4(d, ad, smem_desc_sw128(b + route_bytes / 2 + k * 32), id, sf, sf + 8, 1u);
+          }
+          umma_commit(&done[t % kBars]);
+          if (++cstage == code_stages) cstage = 0;
+          if (++rstage == route_stages) rstage = 0;
         }
         if (!ok) break;
         umma_commit(&tfull[acc]);
@@ -439,123 +561,101 @@ __global__ void __launch_bounds__(kMxThreadsG, 1)
       const uint64_t t0 = globaltimer_ns();
       while (!mbar_try_wait(drain, 0) && globaltimer_ns() - t0 < kMxWaitNs) {}
     }
-  } else if (warp >= 6) {
-    // ---------------- expansion (warps 6..13) ----------------
-    const int set = warp >= 10;            // even or odd steps
-    const int r = (warp & 3) * 32 + lane;  // weight row of the tile = TMEM lane
-    const uint32_t lanes = tmem + kTmemW + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    int cstage = 0, stage = set;
-    uint32_t cphase = 0, phase = 0;
-    bool ok = true;
-    while (ok) {
-      if (!mx_wait_warp(&ifull[q], qphase, abort_flag, p.err)) break;
-      const int item = ring[q];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&iempty[q]);
-      if (++q == kRing) { q = 0; qphase ^= 1; }
-      if (item < 0) break;
-      const int K = item < n_groups * p.mt1 ? p.hidden : p.inter;
-      for (int k0 = 0; k0 < K && ok; k0 += kMxChunkK) {
-        if (!mx_wait_warp(&cfull[cstage], cphase, abort_flag, p.err)) { ok = false; break; }
-        const uint8_t* cs = codes + cstage * kCodeBytes + r * 128;
-        const uint2 sc = *reinterpret_cast<const uint2*>(scale + cstage * kScaleBytes + r * 8);
-        // this warp's one or two steps of the chunk: steps set and set + 2
-        const int n = K - k0 >= kMxChunkK ? 2 : 1;
-        uint4 c[4];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if (i < n) {
-            const int at = 2 * (set + 2 * i);
-            c[2 * i] = *reinterpret_cast<const uint4*>(cs + ((at ^ (r & 7)) << 4));
-            c[2 * i + 1] = *reinterpret_cast<const uint4*>(cs + (((at + 1) ^ (r & 7)) << 4));
-          }
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&cempty[cstage]);  // the codes are in registers
-        if (++cstage == kCodeStages) { cstage = 0; cphase ^= 1; }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if (i < n) {
-            const uint32_t two = (i ? sc.y : sc.x) >> (16 * set);
-            uint32_t o[32];
-            expand32(c[2 * i], two & 255u, o);
-            expand32(c[2 * i + 1], (two >> 8) & 255u, o + 16);
-            if (!mx_wait_warp(&sempty[stage], phase ^ 1, abort_flag, p.err)) { ok = false; break; }
-            tc_fence_after();
-            tmem_st32(lanes + stage * 32, o);
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&wfull[stage]);
-            stage += 2;
-            if (stage >= kSteps) { stage -= kSteps; phase ^= 1; }
-          }
-        }
-      }
-    }
   } else {
-    // ---------------- epilogue (warps 2..5) ----------------
+    // ---------------- epilogue (warps 2..9) ----------------
+    // group 0 drains accumulator 0, group 1 accumulator 1: every other item.
     // TMEM lanes 32 * (warp % 4)..: quarters 0, 1 hold gate rows of a phase-1
     // tile, 2, 3 the up rows of the same features
+    const int eg = (warp - kFirstEpi) >> 2;
     const int qd = warp & 3;
     const bool up_rows = qd >= 2;
     const int f_local = (qd & 1) * 32 + lane;
+    float* xchg = xchg_all[eg];
     float* give = xchg + (up_rows ? kMxFeatures * kXStride : 0) + f_local * kXStride;
     const float* take = xchg + (up_rows ? 0 : kMxFeatures * kXStride) + f_local * kXStride;
-    int acc = 0;
     uint32_t acc_phase = 0;
-    for (;;) {
-      if (!mx_epilogue_all(mx_wait(&ifull[q], qphase, abort_flag, p.err))) break;
-      const int item = ring[q];
+    for (int turn = 0;; turn ^= 1) {
+      if (!mx_epilogue_all(eg, mx_wait(&ifull[q], qphase, abort_flag, p.err))) break;
+      const MxItem it = ring[q];
       __syncwarp();
       if (lane == 0) mbar_arrive(&iempty[q]);
       if (++q == kRing) { q = 0; qphase ^= 1; }
-      if (item < 0) break;  // the same entry for all four warps
-      const MxItem it = mx_item(p, n_groups, item);
-      const MxGroup g = p.groups[it.group];
-      if (!mx_epilogue_all(mx_wait(&tfull[acc], acc_phase, abort_flag, p.err))) break;
+      if (it.phase == 0) break;  // the same entry for all four warps
+      if (turn != eg) continue;
+      // routing weights of routes lane, lane + 32, ... (phase 2)
+      float w[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        w[c] = it.bad ? __uint_as_float(0x7fc00000u)
+               : it.phase == 2 && lane + 32 * c < it.count ? p.route_w[it.start + lane + 32 * c] : 0.0f;
+      if (!mx_epilogue_all(eg, mx_wait(&tfull[eg], acc_phase, abort_flag, p.err))) break;
+      acc_phase ^= 1;
       tc_fence_after();
-      const uint32_t d = tmem + (static_cast<uint32_t>(qd * 32) << 16) + acc * kMxN;
+      const uint32_t d = tmem + (static_cast<uint32_t>(qd * 32) << 16) + eg * kMxN;
       if (it.phase == 1) {
         // 32 routes at a time: gate warps finish the first 16, up warps the rest
-        const int column = mx_column(it.tile * kMxFeatures + f_local);
-        for (int c0 = 0; c0 < g.count; c0 += 32) {
+        const int block = it.tile * 2 + (qd & 1);  // of 32 features
+        for (int c0 = 0; c0 < it.count; c0 += 32) {
           float lo[16], hi[16];
           tmem_ld16(d + c0, lo);
           tmem_ld16(d + c0 + 16, hi);
 #pragma unroll
           for (int j = 0; j < 16; ++j) give[j] = up_rows ? lo[j] : hi[j];
-          mx_epilogue_sync();
+          mx_epilogue_sync(eg);
           const int first = c0 + (up_rows ? 16 : 0);
+          uint8_t* to = p.act + static_cast<int64_t>(it.start + first) * (2 * p.inter) + it.tile * kMxFeatures +
+                        f_local;
+          uint8_t* sb = p.as + static_cast<int64_t>(it.start + first) * p.pitch2 + block;
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            if (first + j < g.count) {
-              const float gate = up_rows ? take[j] : lo[j];
-              const float up = up_rows ? hi[j] : take[j];
-              const float a = __fdividef(gate, 1.0f + __expf(-gate)) * up;
-              p.act[static_cast<size_t>(g.start + first + j) * p.inter + column] = __float2bfloat16_rn(a);
+          for (int j = 0; j < 16; j += 2) {
+            if (first + j < it.count) {  // the same for the whole warp
+              float a[2];
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const float gate = up_rows ? take[j + i] : lo[j + i];
+                const float up = up_rows ? hi[j + i] : take[j + i];
+                a[i] = __fdividef(gate, 1.0f + __expf(-gate)) * up;
+              }
+              int byte[2];
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(a[i]) & 0x7fffffffu);
+                byte[i] = mx_block_byte(top >> 23);
+                a[i] *= mx_block_mult(byte[i]);
+              }
+              uint32_t h, l;
+              mx_split2(a[0], a[1], &h, &l);
+              to[0] = static_cast<uint8_t>(h);
+              to[p.inter] = static_cast<uint8_t>(l);
+              if (lane == 0) sb[0] = static_cast<uint8_t>(byte[0]);
+              if (first + j + 1 < it.count) {
+                to[2 * p.inter] = static_cast<uint8_t>(h >> 8);
+                to[3 * p.inter] = static_cast<uint8_t>(l >> 8);
+                if (lane == 0) sb[p.pitch2] = static_cast<uint8_t>(byte[1]);
+              }
+              to += 4 * p.inter;
+              sb += 2 * p.pitch2;
             }
           }
-          mx_epilogue_sync();
+          mx_epilogue_sync(eg);
         }
       } else {
-        const int feature = it.tile * kMxM + qd * 32 + lane;
-        for (int c0 = 0; c0 < g.count; c0 += 16) {
+        __nv_bfloat16* to = p.out + static_cast<int64_t>(it.start) * p.hidden + it.tile * kMxM + qd * 32 + lane;
+        for (int c0 = 0; c0 < it.count; c0 += 16) {
           float v[16];
           tmem_ld16(d + c0, v);
+          const float ws = c0 < 32 ? w[0] : c0 < 64 ? w[1] : c0 < 96 ? w[2] : w[3];
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
-            if (c0 + j < g.count) {
-              const size_t row = static_cast<size_t>(g.start + c0 + j);
-              const float w = g.bad ? __uint_as_float(0x7fc00000u) : p.route_w[row];
-              p.out[row * p.hidden + feature] = __float2bfloat16_rn(v[j] * w);
-            }
+            const float wj = __shfl_sync(0xffffffffu, ws, (c0 & 16) + j);
+            if (c0 + j < it.count) *to = __float2bfloat16_rn(v[j] * wj);
+            to += p.hidden;
           }
         }
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&tempty[acc]);
-      if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+      if (lane == 0) mbar_arrive(&tempty[eg]);
       if (it.phase == 1) {
         // publish this warp's activations to the sub-group's phase-2 items
         __threadfence();
@@ -575,8 +675,8 @@ __global__ void __launch_bounds__(kMxThreadsG, 1)
 
 // ---------------------------------------------------------------------------
 // Before the GEMM, one launch: block 0 turns the groups into sub-groups and
-// zeroes the counters; the other blocks gather the routes' rows (columns in the
-// stored order) and weights, a warp per route.
+// zeroes the counters; the other blocks gather the routes' rows as hi and lo
+// parts, their scales and weights, a warp per route.
 struct MxPrepare {
   const int64_t* slots;
   const int64_t* starts;
@@ -589,12 +689,12 @@ struct MxPrepare {
   const void* weights;
   int weights_type;
   int64_t topk;
-  int hidden;
-  __nv_bfloat16* x;
+  int hidden, pitch1;
+  uint8_t* x;   // [routes, 2 * hidden]
+  uint8_t* xs;  // [routes, pitch1]
   float* route_w;
   MxGroup* groups;
-  int* n_sub;
-  int* queue;
+  MxHeader* header;
   int* dep;
   int* err;
 };
@@ -606,29 +706,43 @@ __global__ void __launch_bounds__(kPrepThreads) mxfp4_prepare_kernel(const MxPre
   if (blockIdx.x == 0) {
     __shared__ int warp_sum[kPrepThreads / 32];
     __shared__ int base;
-    if (threadIdx.x == 0) { base = 0; *a.queue = 0; }
     // ascending starts inside [0, routes], or no group at all: the tables below
     // are sized for groups that do not overlap
     bool ordered = true;
+    int active = 0;
     for (int g = threadIdx.x; g <= a.n_groups; g += kPrepThreads) {
-      const int64_t s0 = a.starts[g];
-      ordered &= s0 >= 0 && s0 <= a.routes && (g == 0 || a.starts[g - 1] <= s0);
+      const int64_t s0 = a.starts[g], before = g == 0 ? 0 : a.starts[g - 1];
+      ordered &= s0 >= before && s0 <= a.routes;
+      active += g > 0 && s0 > before;
     }
-    if (!__syncthreads_and(ordered)) {
-      if (threadIdx.x == 0) { *a.n_sub = 0; atomicCAS(a.err, 0, DEV_BAD_INPUT); }
+    if (threadIdx.x == 0) { base = 0; a.header->queue = 0; }
+    ordered = __syncthreads_and(ordered);
+    if (!ordered) {
+      if (threadIdx.x == 0) { a.header->n_groups = 0; a.header->box = 0; atomicCAS(a.err, 0, DEV_BAD_INPUT); }
       return;
     }
+    atomicAdd(&base, active);
+    __syncthreads();
+    active = base;
+    __syncthreads();
+    if (threadIdx.x == 0) base = 0;
+    // sub-groups no wider than the mean group asks for, in one of four sizes
+    const int64_t all = a.starts[a.n_groups] - a.starts[0];
+    const int64_t mean = active ? (all + active - 1) / active : 0;
+    const int cap = mean <= 4 ? 16 : mean <= 24 ? 32 : mean <= 48 ? 64 : 128;
+    __syncthreads();
     for (int g0 = 0; g0 < a.n_groups; g0 += kPrepThreads) {
       const int g = g0 + threadIdx.x;
-      int64_t s0 = 0, count = 0, slot = 0;
+      int s0 = 0, count = 0;
+      int64_t slot = 0;
       if (g < a.n_groups) {
-        s0 = a.starts[g];
-        count = a.starts[g + 1] - s0;
+        s0 = static_cast<int>(a.starts[g]);
+        count = static_cast<int>(a.starts[g + 1]) - s0;
         slot = a.slots[g];
       }
       const bool bad = count > 0 && (slot < 0 || slot >= a.cache_slots);
       if (bad) { slot = 0; atomicCAS(a.err, 0, DEV_BAD_INPUT); }
-      const int n = static_cast<int>((count + kMxN - 1) / kMxN);
+      const int n = (count + cap - 1) / cap;
       int scan = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -640,17 +754,21 @@ __global__ void __launch_bounds__(kPrepThreads) mxfp4_prepare_kernel(const MxPre
       int before = base;
       for (int w = 0; w < warp; ++w) before += warp_sum[w];
       const int at = before + scan - n;
-      for (int i = 0; i < n; ++i) {
-        const int64_t r0 = count * i / n, r1 = count * (i + 1) / n;
-        a.groups[at + i] = MxGroup{static_cast<int>(slot), static_cast<int>(s0 + r0),
-                                   static_cast<int>(r1 - r0), bad ? 1 : 0};
+      // parts of count / n routes, the first count % n of them one longer
+      for (int i = 0, r = s0; i < n; ++i) {
+        const int len = count / n + (i < count % n);
+        a.groups[at + i] = MxGroup{static_cast<int>(slot), r, len, bad ? 1 : 0};
         a.dep[at + i] = 0;
+        r += len;
       }
       __syncthreads();
       if (threadIdx.x == kPrepThreads - 1) base = before + scan;
       __syncthreads();
     }
-    if (threadIdx.x == 0) *a.n_sub = base;
+    if (threadIdx.x == 0) {
+      a.header->n_groups = base;
+      a.header->box = cap == 16 ? 0 : cap == 32 ? 1 : cap == 64 ? 2 : 3;
+    }
     return;
   }
   // routes outside [starts[0], starts[n_groups]) belong to no group
@@ -674,50 +792,95 @@ __global__ void __launch_bounds__(kPrepThreads) mxfp4_prepare_kernel(const MxPre
       a.route_w[i] = w;
     }
     const uint4* from = reinterpret_cast<const uint4*>(a.input + (good ? row : 0) * a.input_stride);
-    uint4* to = reinterpret_cast<uint4*>(a.x + i * a.hidden);
-    for (int v = lane; v < a.hidden / 8; v += 32) {
+    uint2* to = reinterpret_cast<uint2*>(a.x + i * 2 * a.hidden);
+    uint8_t* sb = a.xs + i * a.pitch1;
+    // 8 values a lane, a block of 32 in four neighbours (hidden is a multiple of
+    // 128: whole blocks, and the lanes of a block are all in or all out)
+    for (int v0 = 0; v0 < a.hidden / 8; v0 += 32) {
+      const int v = v0 + lane;
+      const bool in = v < a.hidden / 8;
       uint4 e = make_uint4(0, 0, 0, 0);
-      if (good) e = from[v];
-      to[v] = make_uint4(__byte_perm(e.x, e.z, 0x5410), __byte_perm(e.x, e.z, 0x7632),
-                         __byte_perm(e.y, e.w, 0x5410), __byte_perm(e.y, e.w, 0x7632));
+      if (in && good) e = from[v];
+      const uint32_t m = __vmaxu2(__vmaxu2(e.x & 0x7fff7fffu, e.y & 0x7fff7fffu),
+                                  __vmaxu2(e.z & 0x7fff7fffu, e.w & 0x7fff7fffu));
+      uint32_t top = max(m & 0xffffu, m >> 16);
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const int byte = mx_block_byte(top >> 7);
+      const float mult = mx_block_mult(byte);
+      const uint32_t in8[4] = {e.x, e.y, e.z, e.w};
+      uint32_t h[4], l[4];
+#pragma unroll
+      for (int i2 = 0; i2 < 4; ++i2)
+        mx_split2(__uint_as_float(in8[i2] << 16) * mult, __uint_as_float(in8[i2] & 0xffff0000u) * mult,
+                  &h[i2], &l[i2]);
+      if (in) {
+        to[v] = make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+        to[a.hidden / 8 + v] = make_uint2(l[0] | (l[1] << 16), l[2] | (l[3] << 16));
+        if ((v & 3) == 0) sb[v >> 2] = static_cast<uint8_t>(byte);
+      }
     }
   }
 }
 
 // ---------------------------------------------------------------------------
 // Host side
-static int make_map_codes(CUtensorMap* map, const void* base, uint64_t row_codes, uint64_t rows,
+// Codes of a weight matrix in every slot: [slots, rows, cols] 4-bit elements,
+// unpacked on the way (16 codes to 16 bytes of shared memory, 8 of them data).
+static int make_map_codes(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows,
                           uint64_t slots, uint64_t slot_bytes, uint32_t box_rows) {
   PFN_encodeTiled enc = encode_tiled_fn();
   if (!enc) return fail(FERRYB_ECUDA, "cuTensorMapEncodeTiled is unavailable");
-  cuuint64_t dims[3] = {row_codes, rows, slots};
-  cuuint64_t strides[2] = {row_codes, slot_bytes};
-  cuuint32_t box[3] = {128, box_rows, 1};
+  cuuint64_t dims[3] = {cols, rows, slots};
+  cuuint64_t strides[2] = {cols / 2, slot_bytes};
+  cuuint32_t box[3] = {kStepK, box_rows, 1};
   cuuint32_t elem[3] = {1, 1, 1};
-  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box,
-                   elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, 3, const_cast<void*>(base), dims, strides,
+                   box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     return fail(FERRYB_ECUDA, "cuTensorMapEncodeTiled failed (%d) for %llu x %llu codes", (int)r,
-                (unsigned long long)rows, (unsigned long long)row_codes);
+                (unsigned long long)rows, (unsigned long long)cols);
+  return FERRYB_OK;
+}
+
+// Rows of bytes, boxes of 128 bytes x box_rows.
+static int make_map_bytes(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols,
+                          uint32_t box_rows) {
+  PFN_encodeTiled enc = encode_tiled_fn();
+  if (!enc) return fail(FERRYB_ECUDA, "cuTensorMapEncodeTiled is unavailable");
+  cuuint64_t dims[2] = {cols, rows};
+  cuuint64_t strides[1] = {cols};
+  cuuint32_t box[2] = {kStepK, box_rows};
+  cuuint32_t elem[2] = {1, 1};
+  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box,
+                   elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(FERRYB_ECUDA, "cuTensorMapEncodeTiled failed (%d) for %llu x %llu bytes", (int)r,
+                (unsigned long long)rows, (unsigned long long)cols);
   return FERRYB_OK;
 }
 
 static int64_t mx_align(int64_t b) { return (b + 255) & ~int64_t(255); }
 
 struct MxWs {
-  int64_t x, act, w, groups, counters, total;
-  int64_t max_sub;
+  int64_t x, xs, act, as, w, groups, header, total;
+  int64_t pitch1, pitch2, max_sub;
 };
 static MxWs mx_ws(int64_t routes, int64_t n_groups, int64_t hidden, int64_t inter) {
   MxWs w{};
-  w.max_sub = n_groups + routes / kMxN + 1;
+  w.max_sub = n_groups + routes / 16 + 1;
+  w.pitch1 = (hidden / 32 + 15) & ~int64_t(15);
+  w.pitch2 = (inter / 32 + 15) & ~int64_t(15);
   w.x = 0;
-  w.act = w.x + mx_align(routes * hidden * 2);
-  w.w = w.act + mx_align(routes * inter * 2);
+  w.xs = w.x + mx_align(routes * hidden * 2);
+  w.act = w.xs + mx_align(routes * w.pitch1);
+  w.as = w.act + mx_align(routes * inter * 2);
+  w.w = w.as + mx_align(routes * w.pitch2);
   w.groups = w.w + mx_align(routes * 4);
-  w.counters = w.groups + mx_align(w.max_sub * (int64_t)sizeof(MxGroup));
-  w.total = w.counters + mx_align((2 + w.max_sub) * 4);
+  w.header = w.groups + mx_align(w.max_sub * (int64_t)sizeof(MxGroup));
+  w.total = w.header + 256 + mx_align(w.max_sub * 4);  // then the dependency counters
   return w;
 }
 
@@ -735,7 +898,7 @@ static int mx_sizes(int64_t routes, int64_t n_groups, int64_t hidden, int64_t in
                "execute_experts_mxfp4: %lld routes in %lld groups", (long long)routes,
                (long long)n_groups);
   // the work counter is 32 bits
-  FB_CHECK_ARG((n_groups + routes / kMxN + 1) * (inter / 64 + hidden / 128) < (int64_t(1) << 30),
+  FB_CHECK_ARG((n_groups + routes / 16 + 1) * (inter / 64 + hidden / 128) < (int64_t(1) << 30),
                "execute_experts_mxfp4: too many work items");
   return FERRYB_OK;
 }
@@ -758,17 +921,16 @@ extern "C" int ferryb_execute_experts_mxfp4(const ferryb_mxfp4_experts_args* e, 
   FB_CHECK_ARG(e->n_input >= 0 && e->topk >= 0, "execute_experts_mxfp4: bad input sizes");
   FB_CHECK_ARG(e->weights_type >= FERRYB_BF16 && e->weights_type <= FERRYB_FP32,
                "execute_experts_mxfp4: unknown weights type %d", e->weights_type);
-  FB_CHECK_ARG(reinterpret_cast<uintptr_t>(e->cache) % 16 == 0 &&
+  FB_CHECK_ARG(reinterpret_cast<uintptr_t>(e->cache) % 32 == 0 &&
                    reinterpret_cast<uintptr_t>(e->input) % 16 == 0 &&
                    (e->n_input <= 1 || (e->input_stride % 8 == 0 && e->input_stride >= e->hidden)),
-               "execute_experts_mxfp4: cache and input rows must be 16-byte aligned");
+               "execute_experts_mxfp4: the cache must be 32-byte, input rows 16-byte aligned");
   const MxWs ws = mx_ws(e->routes, e->n_groups, e->hidden, e->intermediate);
   FB_CHECK_ARG(e->workspace && reinterpret_cast<uintptr_t>(e->workspace) % 256 == 0 &&
                    e->workspace_bytes >= ws.total,
                "execute_experts_mxfp4: workspace too small (%lld < %lld) or misaligned",
                (long long)e->workspace_bytes, (long long)ws.total);
   uint8_t* base = static_cast<uint8_t*>(e->workspace);
-  int* counters = reinterpret_cast<int*>(base + ws.counters);
 
   MxPrepare pr{};
   pr.slots = e->slots;
@@ -785,48 +947,47 @@ extern "C" int ferryb_execute_experts_mxfp4(const ferryb_mxfp4_experts_args* e, 
   pr.weights_type = e->weights_type;
   pr.topk = e->topk;
   pr.hidden = static_cast<int>(e->hidden);
-  pr.x = reinterpret_cast<__nv_bfloat16*>(base + ws.x);
+  pr.pitch1 = static_cast<int>(ws.pitch1);
+  pr.x = base + ws.x;
+  pr.xs = base + ws.xs;
   pr.route_w = reinterpret_cast<float*>(base + ws.w);
   pr.groups = reinterpret_cast<MxGroup*>(base + ws.groups);
-  pr.queue = counters;
-  pr.n_sub = counters + 1;
-  pr.dep = counters + 2;
+  pr.header = reinterpret_cast<MxHeader*>(base + ws.header);
+  pr.dep = reinterpret_cast<int*>(base + ws.header + 256);
   pr.err = e->err;
 
   int device = 0;
   FB_CUDA(cudaGetDevice(&device));
   const int sms = num_sms(device);
-  CUtensorMap w1, w2;
-  BMaps bx, ba;
+  MxMaps maps;
   const int64_t hi = e->hidden * e->intermediate, row_bytes = 3 * hi / 32 * 17;
   const uint8_t* cache = static_cast<const uint8_t*>(e->cache);
-  if ((s = make_map_codes(&w1, cache, e->hidden / 2, 2 * e->intermediate, e->cache_slots, row_bytes,
+  if ((s = make_map_codes(&maps.w1, cache, e->hidden, 2 * e->intermediate, e->cache_slots, row_bytes,
                           kMxFeatures)))
     return s;
-  if ((s = make_map_codes(&w2, cache + hi, e->intermediate / 2, e->hidden, e->cache_slots, row_bytes,
+  if ((s = make_map_codes(&maps.w2, cache + hi, e->intermediate, e->hidden, e->cache_slots, row_bytes,
                           kMxM)))
     return s;
-  for (int i = 0; i < 4; ++i) {
-    if ((s = make_map_2d_bf16(&bx.m[i], base + ws.x, e->routes, e->hidden, e->hidden * 2, 16u << i,
-                              kMxStepK)))
-      return s;
-    if ((s = make_map_2d_bf16(&ba.m[i], base + ws.act, e->routes, e->intermediate,
-                              e->intermediate * 2, 16u << i, kMxStepK)))
-      return s;
-  }
+  if ((s = make_map_bytes(&maps.x16, base + ws.x, e->routes, 2 * e->hidden, 16))) return s;
+  if ((s = make_map_bytes(&maps.x64, base + ws.x, e->routes, 2 * e->hidden, 64))) return s;
+  if ((s = make_map_bytes(&maps.a16, base + ws.act, e->routes, 2 * e->intermediate, 16))) return s;
+  if ((s = make_map_bytes(&maps.a64, base + ws.act, e->routes, 2 * e->intermediate, 64))) return s;
   MxParams p{};
   p.groups = pr.groups;
-  p.n_groups = pr.n_sub;
+  p.header = pr.header;
   p.mt1 = static_cast<int>(e->intermediate / kMxFeatures);
   p.mt2 = static_cast<int>(e->hidden / kMxM);
   p.hidden = static_cast<int>(e->hidden);
   p.inter = static_cast<int>(e->intermediate);
   p.scales = cache + 3 * hi / 2;
   p.row_bytes = row_bytes;
-  p.act = reinterpret_cast<__nv_bfloat16*>(base + ws.act);
+  p.xs = pr.xs;
+  p.act = base + ws.act;
+  p.as = base + ws.as;
+  p.pitch1 = pr.pitch1;
+  p.pitch2 = static_cast<int>(ws.pitch2);
   p.out = static_cast<__nv_bfloat16*>(e->out);
   p.route_w = pr.route_w;
-  p.queue = pr.queue;
   p.dep = pr.dep;
   p.err = e->err;
 
@@ -840,10 +1001,9 @@ extern "C" int ferryb_execute_experts_mxfp4(const ferryb_mxfp4_experts_args* e, 
                                  (int)kMxSmem));
     if (device < 64) attr_set[device].store(true, std::memory_order_release);
   }
-  const int64_t subs = e->n_groups < e->routes ? e->n_groups + e->routes / kMxN : e->routes;
+  const int64_t subs = e->n_groups < e->routes ? e->n_groups + e->routes / 16 : e->routes;
   const int64_t items = subs * (p.mt1 + p.mt2);
-  mxfp4_swiglu_kernel<<<static_cast<int>(items < sms ? items : sms), kMxThreadsG, kMxSmem, stream>>>(
-      w1, w2, bx, ba, p);
+  mxfp4_swiglu_kernel<<<static_cast<int>(items < sms ? items : sms), kMxThreads, kMxSmem, stream>>>(maps, p);
   FB_LAUNCH_CHECK();
   return FERRYB_OK;
 }

@@ -314,8 +314,8 @@ def execute_experts_mxfp4(cache, input, routing_weights, slots, starts, rows, co
                  cols=cols, out=out, err=err)
     row_bytes = 3 * hidden * intermediate // 32 * 17
     _check(cache.dtype == torch.uint8 and cache.dim() == 2 and cache.shape[1] == row_bytes
-           and cache.is_contiguous() and cache.data_ptr() % 16 == 0,
-           f'cache must be contiguous 16-byte aligned uint8 [slots, {row_bytes}]')
+           and cache.is_contiguous() and cache.data_ptr() % 32 == 0,
+           f'cache must be contiguous 32-byte aligned uint8 [slots, {row_bytes}]')
     _check(input.dtype == BF16 and input.dim() == 2 and input.shape[1] == hidden,
            f'input must be bf16 [n, {hidden}]')
     _check(routing_weights.dim() == 2 and routing_weights.shape[0] == input.shape[0]

@@ -158,10 +158,15 @@ def _run(d, **kw):
 
 def _want(d):
     """(values, bound): the definition in float64 and how far a kernel may be
-    from it that sums in float32, rounds the activation and the result to bf16
-    (half a step each: 2^-8 of the value) and takes exp with the error that
-    CUDA's documentation gives for __expf (2 + 1.173 |x| units of 2^-23, three
-    more for the sum and the quotient, one for the product)."""
+    from it that holds x and the activation as two e4m3 parts (x exactly, the
+    activation within 2^-9 of its value, both within 2^-21 of the largest value
+    of their block of 32 where that is more), sums in float32, rounds the result
+    to bf16 (2^-8 of the value) and takes exp with the error that CUDA's
+    documentation gives for __expf (2 + 1.173 |x| units of 2^-23, three more for
+    the sum and the quotient, one for the product)."""
+    def largest(v):
+        b = np.abs(v).reshape(v.shape[0], -1, 32).max(2, keepdims=True)
+        return np.broadcast_to(b, b.shape[:2] + (32,)).reshape(v.shape)
     H, I = d['hidden'], d['inter']
     x, w = d['x'].double().numpy(), d['w'].double().numpy()
     n = 3 * H * I
@@ -178,13 +183,14 @@ def _want(d):
         gt, u = xs @ gate, xs @ up
         silu = gt / (1 + np.exp(-gt))
         act = silu * u
-        # a float32 sum of H products of bf16 numbers (exact): H - 1 roundings at most
-        dg, du = H * u24 * (np.abs(xs) @ np.abs(gate)), H * u24 * (np.abs(xs) @ np.abs(up))
+        # a float32 sum of 2 H products (exact): 2 H - 1 roundings at most
+        dx = np.where(np.abs(xs) < 2.0 ** -13 * largest(xs), 2.0 ** -21 * largest(xs), 0.0)
+        dg, du = ((2 * H * u24 * (np.abs(xs) + dx) + dx) @ np.abs(m) for m in (gate, up))
         dact = 1.1 * dg * (np.abs(u) + du) + np.abs(silu) * du + (8 + 1.173 * np.abs(gt)) * 2.0 ** -23 * np.abs(act)
-        dact = dact + 2.0 ** -8 * (np.abs(act) + dact)
+        dact = dact + 2.0 ** -9 * (np.abs(act) + dact) + 2.0 ** -21 * largest(np.abs(act) + dact)
         y = act @ down
         wt = w[d['rows'][a:b].numpy(), d['cols'][a:b].numpy()][:, None]
-        dy = (dact + I * u24 * (np.abs(act) + dact)) @ np.abs(down)
+        dy = (dact + 2 * I * u24 * (np.abs(act) + dact)) @ np.abs(down)
         out[a:b] = y * wt
         bound[a:b] = np.abs(wt) * (dy + u24 * (np.abs(y) + dy))
         bound[a:b] += 2.0 ** -8 * (np.abs(out[a:b]) + bound[a:b])
