@@ -31,15 +31,15 @@
 // Data flow of a step (128 columns): TMA unpacks the codes of 128 weight rows
 // into 16 KB of shared memory (4-bit data in 8-bit places, 128-byte swizzle, as
 // the MMA reads them) and brings the routes' hi and lo parts; cp.async brings
-// the weight rows' 4 scale bytes each (pieces of 4 bytes need no padding of the
-// scale rows); four warps move the scales of both sides into tensor memory
+// the weight rows' scale bytes, 4 a step, in pieces of 16, 8 or 4 as the rows are
+// aligned (no padding of the scale rows); four warps move the scales of both sides into tensor memory
 // (row r in lane r % 32 of every 32-lane quarter, column r / 32, one byte for
 // each 32 columns of the step); one thread issues the 8 MMAs of K = 32, hi and
 // lo for each scale byte.
 //
-// CTA roles (480 threads): warp 0 claims work and loads codes and scales; warp
-// 1 issues the MMAs; warps 2-5 and 6-9 drain the two accumulators; warp 10
-// loads the routes; warps 11-14 move the scales.  Codes do not depend on phase
+// CTA roles (512 threads): warp 0 claims work and loads codes; warp 1 issues the
+// MMAs; warps 2-5 and 6-9 drain the two accumulators; warp 10 loads the routes;
+// warp 15 brings the weights' scales, warps 11-14 move all scales on.  Codes do not depend on phase
 // 1, so warp 0 runs ahead into phase 2 while the routes' warps wait for the
 // activations.
 #include <cuda_fp16.h>
@@ -52,24 +52,27 @@
 
 namespace ferryb {
 
-constexpr int kMxWarps = 15;
+constexpr int kMxWarps = 16;
 constexpr int kMxThreads = kMxWarps * 32;
-constexpr int kFirstEpi = 2, kRouteWarp = 10, kFirstScale = 11;
+constexpr int kFirstEpi = 2, kRouteWarp = 10, kFirstScale = 11, kScaleLoad = 15;
 constexpr int kMxM = 128;          // weight rows per tile
 constexpr int kMxN = 128;          // most routes of a sub-group
 constexpr int kStepK = 128;        // columns per step
 constexpr int kMxFeatures = 64;    // gate (= up) rows per phase-1 tile
 constexpr int kBars = 16;          // barriers of the step pipeline, more than any buffer's depth
-constexpr int kScaleStages = 8;    // steps whose scales tensor memory holds
+constexpr int kBlock = 4;          // steps whose scales come in one piece and are arranged by one warp
+constexpr int kTiles = 6;          // steps whose arranged scales shared memory holds
+constexpr int kPieces = 3;         // pieces of scales in shared memory, weights' and routes'
 constexpr uint32_t kCodeBytes = kMxM * kStepK;  // unpacked
-constexpr uint32_t kScaleBytes = kMxM * 4;
-constexpr uint32_t kTmemScale = 256;  // first TMEM column of the scales, 16 a step
+constexpr uint32_t kPieceBytes = kMxM * 16;  // of up to four steps
+constexpr uint32_t kTileBytes = 3 * 512;  // scales of the weights, of the routes, lo scales of 128 routes
+constexpr uint32_t kTmemScale = 256;  // first TMEM column of the scales: four places of 16 columns
 constexpr int kRing = 4;           // claimed items in flight
-constexpr int kXStride = 17;       // floats a feature of the gate/up exchange (padded)
+constexpr int kXStride = 9;        // floats a feature of the gate/up exchange (padded)
 constexpr uint32_t kXchgBytes = 2 * kMxFeatures * kXStride * 4;  // an epilogue group's
 constexpr uint32_t kPoolBytes = 12 * 16384;  // codes and routes
-constexpr int kMaxCodeStages = 10;
-constexpr uint32_t kMxSmem = kPoolBytes + kMaxCodeStages * kScaleBytes + 1024 + 1024;
+constexpr uint32_t kMxSmem = kPoolBytes + 2 * kPieces * kPieceBytes + kTiles * kTileBytes + 1024 +
+                             1024;
 constexpr uint64_t kMxWaitNs = 2000000000ull;  // bound on any wait
 
 // Up to 128 routes of one group.
@@ -94,10 +97,9 @@ struct MxParams {
   int hidden, inter;
   const uint8_t* scales;  // slot 0's scale bytes
   int64_t row_bytes;      // bytes of a cache row
-  const uint8_t* xs;      // hi scale bytes of the routes [routes, pitch1]
   uint8_t* act;           // [routes, 2 * I]: hi, lo
   uint8_t* as;            // hi scale bytes of the activations [routes, pitch2]
-  int pitch1, pitch2;
+  int pitch2;
   __nv_bfloat16* out;
   const float* route_w;
   int* dep;    // [sub-groups] phase-1 epilogue-warp completions, zero at launch
@@ -108,6 +110,7 @@ struct MxMaps {
   CUtensorMap w1, w2;        // codes of gate and up rows (64-row boxes), of down rows (128)
   CUtensorMap x16, x64;      // routes [routes, 2 * H], boxes of 16 and 64 rows
   CUtensorMap a16, a64;      // activations [routes, 2 * I]
+  CUtensorMap xs, as;        // their scale bytes [routes, pitch], boxes of 16 x 16
 };
 
 // A claimed work item, handed from warp 0 to the other roles.
@@ -184,8 +187,10 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, u
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
       : "memory");
 }
-__device__ __forceinline__ void cp_async4(void* dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+template <int BYTES>
+__device__ __forceinline__ void cp_async(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(dst)), "l"(src), "n"(BYTES)
+               : "memory");
 }
 // Arrive on `bar` once this thread's cp.async copies so far have landed (the
 // barrier's count includes this arrival).
@@ -193,14 +198,26 @@ __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
-// 32 lanes x 4 columns of 32 bits into tensor memory.
-__device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint32_t* r) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(r[0]),
-               "r"(r[1]), "r"(r[2]), "r"(r[3])
-               : "memory");
+// 32 rows of 16 bytes of shared memory (rows one after the other) into 4 columns
+// of every 32-lane quarter of tensor memory.  Ordered before the MMAs that the
+// same thread issues after it.
+__device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint32_t saddr) {
+  // descriptor: address >> 4, 8-row groups 128 bytes apart (bits 32-45), version
+  // 1 (bits 46-47), no swizzle
+  const uint64_t desc = static_cast<uint64_t>((saddr >> 4) & 0x3FFF) | (static_cast<uint64_t>(1) << 16) |
+                        (static_cast<uint64_t>(128 >> 4) << 32) | (static_cast<uint64_t>(1) << 46);
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
-__device__ __forceinline__ void tmem_st_wait() {
-  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+// 32 lanes x 8 consecutive columns of 32 bits.
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, float* v) {
+  uint32_t r[8];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+                 "=r"(r[7])
+               : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
 }
 
 // D[tmem] (+)= (A[smem] * scales) x (B[smem] * scales)^T, 32 columns: e2m1 codes
@@ -274,6 +291,11 @@ __host__ __device__ __forceinline__ int mx_route_stages(int box) {
 }
 __host__ __device__ __forceinline__ uint32_t mx_route_bytes(int box) { return (16u << box) * kStepK * 2; }
 
+// Rows of routes that a sub-group's tile holds: 16, 32, 64 or 128.
+__device__ __forceinline__ int mx_rows(int count) {
+  return count <= 16 ? 16 : count <= 32 ? 32 : count <= 64 ? 64 : 128;
+}
+
 // Steps are numbered from 0 over all items of a CTA.  Step t uses barrier t % 16
 // of each pipeline; a buffer of S stages may be refilled for step t once step
 // t - S is done, and S < 16 keeps the parity unambiguous.
@@ -281,6 +303,10 @@ __device__ __forceinline__ bool mx_wait_step(uint64_t* bars, uint32_t t, volatil
                                              int* err) {
   return mx_wait(bars + t % kBars, (t / kBars) & 1, abort_flag, err);
 }
+
+// Scale bytes of a row that are copied at once (16, 8 or 4): rows of K / 32 bytes
+// start on multiples of the widest of them that divides the row.
+__device__ __forceinline__ int mx_piece(int K) { return K % 512 == 0 ? 16 : K % 256 == 0 ? 8 : 4; }
 
 // Wait until the sub-group's activations are written: four epilogue warps for
 // each of its phase-1 tiles.
@@ -306,11 +332,16 @@ __global__ void __launch_bounds__(kMxThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
-  uint8_t* scale = smem + kPoolBytes;  // [code stages][128 rows] 4 scale bytes
-  uint64_t* full = reinterpret_cast<uint64_t*>(scale + kMaxCodeStages * kScaleBytes);
-  uint64_t* kfull = full + kBars;    // the weights' scale bytes landed
-  uint64_t* done = kfull + kBars;    // the MMAs of a step are complete
-  uint64_t* tfull = done + kBars;    // [2] accumulators
+  uint8_t* scale = smem + kPoolBytes;  // [pieces][128 rows] 16 scale bytes
+  uint8_t* rscale = scale + kPieces * kPieceBytes;  // the same of the routes
+  uint8_t* tiles = rscale + kPieces * kPieceBytes;  // [kTiles] arranged scales
+  uint64_t* full = reinterpret_cast<uint64_t*>(tiles + kTiles * kTileBytes);
+  uint64_t* done = full + kBars;     // the MMAs of a step are complete
+  uint64_t* kfull = done + kBars;    // [kPieces] weight scales landed
+  uint64_t* kempty = kfull + kPieces;
+  uint64_t* bfull = kempty + kPieces;  // [kPieces] route scales landed
+  uint64_t* bempty = bfull + kPieces;
+  uint64_t* tfull = bempty + kPieces;  // [2] accumulators
   uint64_t* tempty = tfull + 2;
   uint64_t* ifull = tempty + 2;      // [kRing] claimed items
   uint64_t* iempty = ifull + kRing;
@@ -323,12 +354,17 @@ __global__ void __launch_bounds__(kMxThreads, 1)
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (threadIdx.x == 0) {
     for (int s = 0; s < kBars; ++s) {
-      mbar_init(&full[s], 6);    // codes, routes and four scale warps
-      mbar_init(&kfull[s], 32);  // cp.async of warp 0's lanes
+      mbar_init(&full[s], 3);  // codes, routes and scales
       mbar_init(&done[s], 1);
     }
+    for (int s = 0; s < kPieces; ++s) {
+      mbar_init(&kfull[s], 32);
+      mbar_init(&kempty[s], 4);
+      mbar_init(&bfull[s], 1);
+      mbar_init(&bempty[s], 4);
+    }
     for (int b = 0; b < 2; ++b) { mbar_init(&tfull[b], 1); mbar_init(&tempty[b], 4); }
-    for (int q = 0; q < kRing; ++q) { mbar_init(&ifull[q], 1); mbar_init(&iempty[q], 14); }
+    for (int q = 0; q < kRing; ++q) { mbar_init(&ifull[q], 1); mbar_init(&iempty[q], 15); }
     mbar_init(drain, 1);
     *abort_flag = 0;
     fence_barrier_init();
@@ -346,36 +382,33 @@ __global__ void __launch_bounds__(kMxThreads, 1)
   uint32_t qphase = 0;
 
   if (warp == 0) {
-    // ---------------- claims, codes and scales ----------------
-    uint32_t t = 0, stage = 0;
-    bool ok = true;
-    const int n_groups = p.header->n_groups;
-    int next = lane == 0 ? atomicAdd(&p.header->queue, 1) : 0;
-    while (ok) {
-      const MxItem it = mx_item(p, n_groups, __shfl_sync(0xffffffffu, next, 0));
-      if (!mx_wait_warp(&iempty[q], qphase ^ 1, abort_flag, p.err)) { ok = false; break; }
-      if (lane == 0) {
+    // ---------------- claims and codes ----------------
+    if (elect_one()) {
+      uint32_t t = 0, stage = 0;
+      bool ok = true;
+      const int n_groups = p.header->n_groups;
+      auto publish = [&](const MxItem& it) {
+        if (!mx_wait(&iempty[q], qphase ^ 1, abort_flag, p.err)) return false;
         ring[q] = it;
         mbar_arrive(&ifull[q]);
-      }
-      if (++q == kRing) { q = 0; qphase ^= 1; }
-      if (it.phase == 0) break;
-      if (lane == 0) next = atomicAdd(&p.header->queue, 1);  // back before this item's loads are issued
-      const int K = it.phase == 1 ? p.hidden : p.inter;
-      // scale bytes of the tile rows that this lane copies: lane + 32 * i
-      const int pitch = K / 32;
-      const int row0 = it.tile * (it.phase == 1 ? kMxFeatures : kMxM);
-      const uint8_t* src = p.scales + it.slot * p.row_bytes + static_cast<int64_t>(row0 + lane) * pitch +
-                           (it.phase == 1 ? 0 : 2 * static_cast<int64_t>(p.inter) * (p.hidden / 32));
-      const int64_t d1 = 32 * pitch;
-      const int64_t d2 = it.phase == 1 ? static_cast<int64_t>(p.inter) * pitch : 2 * d1;  // up rows
-      for (int k0 = 0; k0 < K; k0 += kStepK, ++t) {
-        if (t >= code_stages &&
-            !__all_sync(0xffffffffu, mx_wait_step(done, t - code_stages, abort_flag, p.err))) {
-          ok = false;
-          break;
-        }
-        if (lane == 0) {
+        if (++q == kRing) { q = 0; qphase ^= 1; }
+        return true;
+      };
+      MxItem it = mx_item(p, n_groups, atomicAdd(&p.header->queue, 1));
+      ok = publish(it);
+      while (ok && it.phase != 0) {
+        // the next item is claimed now and published a few steps on, before this
+        // one's last loads: its scales and routes are under way in time
+        const int id = atomicAdd(&p.header->queue, 1);
+        MxItem next{};
+        const int K = it.phase == 1 ? p.hidden : p.inter;
+        const int row0 = it.tile * (it.phase == 1 ? kMxFeatures : kMxM);
+        const int ahead = min(K - kStepK, 3 * kStepK);
+        for (int k0 = 0; k0 < K; k0 += kStepK, ++t) {
+          if (t >= code_stages && !mx_wait_step(done, t - code_stages, abort_flag, p.err)) {
+            ok = false;
+            break;
+          }
           uint64_t* bar = full + t % kBars;
           uint8_t* cs = smem + stage * kCodeBytes;
           mbar_expect_tx(bar, kCodeBytes / 2);  // the copy counts its 4-bit data, not the gaps
@@ -385,29 +418,72 @@ __global__ void __launch_bounds__(kMxThreads, 1)
           } else {
             tma_load_3d(cs, &maps.w2, bar, k0, row0, it.slot);
           }
+          if (++stage == code_stages) stage = 0;
+          if (k0 == ahead) {
+            next = mx_item(p, n_groups, id);
+            if (!publish(next)) { ok = false; break; }
+          }
         }
-        uint8_t* ss = scale + stage * kScaleBytes + lane * 4;
-        cp_async4(ss, src);
-        cp_async4(ss + 128, src + d1);
-        cp_async4(ss + 256, src + d2);
-        cp_async4(ss + 384, src + d2 + d1);
-        cp_async_arrive(&kfull[t % kBars]);
-        src += kStepK / 32;
-        if (++stage == code_stages) stage = 0;
+        it = next;
+      }
+      if (!ok) {
+        // the other roles stop at the abort flag; this CTA's loads get a bounded
+        // time to land (a step's barrier may lack another role's arrival now)
+        *abort_flag = 1;
+        const uint64_t t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 1000000) {}
       }
     }
-    if (!ok) {
-      // the other roles stop at the abort flag; this CTA's loads get a bounded
-      // time to land (a step's barrier may lack another role's arrival now)
-      *abort_flag = 1;
-      asm volatile("cp.async.wait_all;" ::: "memory");
-      const uint64_t t0 = globaltimer_ns();
-      while (globaltimer_ns() - t0 < 1000000) {}
+  } else if (warp == kScaleLoad) {
+    // ---------------- weight scales into shared memory ----------------
+    int piece = 0;
+    uint32_t pphase = 0;
+    bool ok = true;
+    while (ok) {
+      if (!mx_wait_warp(&ifull[q], qphase, abort_flag, p.err)) break;
+      const int phase = ring[q].phase, tile = ring[q].tile, slot = ring[q].slot;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&iempty[q]);
+      if (++q == kRing) { q = 0; qphase ^= 1; }
+      if (phase == 0) break;
+      const int K = phase == 1 ? p.hidden : p.inter;
+      // tile rows lane + 32 * i, a piece of 4, 2 or 1 steps (the widest copy
+      // that the rows' alignment allows) each
+      const int pitch = K / 32, width = mx_piece(K);
+      const uint8_t* src = p.scales + slot * p.row_bytes +
+                           (phase == 1 ? 0 : 2 * static_cast<int64_t>(p.inter) * (p.hidden / 32)) +
+                           static_cast<int64_t>(tile * (phase == 1 ? kMxFeatures : kMxM) + lane) * pitch;
+      const int64_t d1 = 32 * pitch;
+      const int64_t d2 = phase == 1 ? static_cast<int64_t>(p.inter) * pitch : 2 * d1;  // up rows
+      for (int b = 0; b < pitch; b += width) {
+        if (!mx_wait_warp(&kempty[piece], pphase ^ 1, abort_flag, p.err)) { ok = false; break; }
+        uint8_t* to = scale + piece * kPieceBytes + lane * 16;
+        if (width == 16) {
+          cp_async<16>(to, src + b);
+          cp_async<16>(to + 512, src + b + d1);
+          cp_async<16>(to + 1024, src + b + d2);
+          cp_async<16>(to + 1536, src + b + d2 + d1);
+        } else if (width == 8) {
+          cp_async<8>(to, src + b);
+          cp_async<8>(to + 512, src + b + d1);
+          cp_async<8>(to + 1024, src + b + d2);
+          cp_async<8>(to + 1536, src + b + d2 + d1);
+        } else {
+          cp_async<4>(to, src + b);
+          cp_async<4>(to + 512, src + b + d1);
+          cp_async<4>(to + 1024, src + b + d2);
+          cp_async<4>(to + 1536, src + b + d2 + d1);
+        }
+        cp_async_arrive(&kfull[piece]);
+        if (++piece == kPieces) { piece = 0; pphase ^= 1; }
+      }
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp == kRouteWarp) {
     // ---------------- routes ----------------
     if (elect_one()) {
-      uint32_t t = 0, stage = 0;
+      uint32_t t = 0, stage = 0, bphase = 0;
+      int piece = 0;
       bool ok = true;
       while (ok) {
         if (!mx_wait(&ifull[q], qphase, abort_flag, p.err)) { ok = false; break; }
@@ -420,13 +496,22 @@ __global__ void __launch_bounds__(kMxThreads, 1)
           asm volatile("fence.proxy.async.global;" ::: "memory");
         }
         const int K = it.phase == 1 ? p.hidden : p.inter;
-        // 16 or 32 rows in boxes of 16, 64 or 128 in boxes of 64
-        const int n = (it.count + 15) & ~15;
+        // 16 or 32 rows in boxes of 16, 64 or 128 in boxes of 64; the lo part's
+        // rows follow the hi part's
+        const int n = mx_rows(it.count);
         const int rows = n <= 32 ? 16 : 64;
-        const int boxes = n <= 32 ? n / 16 : (n + 63) / 64;
+        const int boxes = n / rows;
         const CUtensorMap* map = it.phase == 1 ? (rows == 16 ? &maps.x16 : &maps.x64)
                                                : (rows == 16 ? &maps.a16 : &maps.a64);
+        const CUtensorMap* smap = it.phase == 1 ? &maps.xs : &maps.as;
         for (int k0 = 0; k0 < K; k0 += kStepK, ++t) {
+          if (k0 % (kBlock * kStepK) == 0) {  // the scale bytes of four steps
+            if (!mx_wait(&bempty[piece], bphase ^ 1, abort_flag, p.err)) { ok = false; break; }
+            mbar_expect_tx(&bfull[piece], n * 16);
+            for (int i = 0; i < n; i += 16)
+              tma_load_2d(rscale + piece * kPieceBytes + i * 16, smap, &bfull[piece], k0 / 32, it.start + i);
+            if (++piece == kPieces) { piece = 0; bphase ^= 1; }
+          }
           if (t >= route_stages && !mx_wait_step(done, t - route_stages, abort_flag, p.err)) {
             ok = false;
             break;
@@ -436,7 +521,7 @@ __global__ void __launch_bounds__(kMxThreads, 1)
           mbar_expect_tx(bar, static_cast<uint32_t>(boxes * rows * kStepK * 2));
           for (int i = 0; i < boxes; ++i) {
             tma_load_2d(to + i * rows * kStepK, map, bar, k0, it.start + i * rows);
-            tma_load_2d(to + route_bytes / 2 + i * rows * kStepK, map, bar, K + k0, it.start + i * rows);
+            tma_load_2d(to + (n + i * rows) * kStepK, map, bar, K + k0, it.start + i * rows);
           }
           if (++stage == route_stages) stage = 0;
         }
@@ -448,89 +533,110 @@ __global__ void __launch_bounds__(kMxThreads, 1)
       }
     }
   } else if (warp >= kFirstScale) {
-    // ---------------- scales into tensor memory ----------------
-    // every warp writes the whole set into its own 32-lane quarter
-    const uint32_t mine = tmem + kTmemScale + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    uint32_t t = 0, stage = 0;
+    // ---------------- scales arranged ----------------
+    // Into the MMA's order: row r's four bytes of a step at (r % 32) * 16 + r / 32
+    // * 4.  A block of up to four steps is one warp's, the blocks go around.  All
+    // four warps wait for and release every piece, so that none falls behind a
+    // barrier by more than a phase.
+    uint32_t t = 0, blk = 0, piece = 0, tile = 0;  // counted over all items
     bool ok = true;
     while (ok) {
       if (!mx_wait_warp(&ifull[q], qphase, abort_flag, p.err)) break;
-      const int phase = ring[q].phase, group = ring[q].group, start = ring[q].start, count = ring[q].count;
+      const int phase = ring[q].phase, count = ring[q].count;
       __syncwarp();
       if (lane == 0) mbar_arrive(&iempty[q]);
       if (++q == kRing) { q = 0; qphase ^= 1; }
       if (phase == 0) break;
-      if (phase == 2) {
-        bool there = true;
-        if (lane == 0) there = mx_wait_dep(p.dep + group, 4 * p.mt1, abort_flag, p.err);
-        if (!__shfl_sync(0xffffffffu, there, 0)) break;
-        __syncwarp();  // lane 0's acquire covers the warp's reads
-      }
       const int K = phase == 1 ? p.hidden : p.inter;
-      const int pitch = phase == 1 ? p.pitch1 : p.pitch2;
-      const uint8_t* from = (phase == 1 ? p.xs : p.as) + static_cast<int64_t>(start + lane) * pitch;
-      // the routes' bytes of four steps at a time, fetched one such block ahead
-      uint4 cur[4], nxt[4];
-      auto fetch = [&](int k0, uint4* v) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          v[c] = make_uint4(0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu);
-          if (lane + 32 * c < count)
-            v[c] = __ldcg(reinterpret_cast<const uint4*>(from + static_cast<int64_t>(32 * c) * pitch + k0 / 32));
-        }
-      };
-      fetch(0, nxt);
-      for (int k0 = 0; k0 < K && ok; k0 += 4 * kStepK) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) cur[c] = nxt[c];
-        if (k0 + 4 * kStepK < K) fetch(k0 + 4 * kStepK, nxt);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (k0 + i * kStepK >= K) break;
-          uint32_t hi[4], lo[4], a[4];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            hi[c] = i == 0 ? cur[c].x : i == 1 ? cur[c].y : i == 2 ? cur[c].z : cur[c].w;
-            lo[c] = hi[c] - 0x04040404u;  // every byte is at least 4
+      const int per_piece = mx_piece(K) / 4;  // steps
+      const int rows = mx_rows(count);
+      const int mine = rows == 16 ? lane & 15 : lane;
+      for (int k0 = 0; k0 < K && ok; k0 += kBlock * kStepK, ++blk) {
+        const int n = min(kBlock, (K - k0) / kStepK);
+        const uint32_t rp = blk % kPieces;
+        const uint32_t* rs = reinterpret_cast<const uint32_t*>(rscale + rp * kPieceBytes);
+        if (!mx_wait_warp(&bfull[rp], (blk / kPieces) & 1, abort_flag, p.err)) { ok = false; break; }
+        if ((blk & 3) != static_cast<uint32_t>(warp - kFirstScale)) {
+          if (lane == 0) mbar_arrive(&bempty[rp]);
+          for (int i = 0; i < n && ok; i += per_piece, ++piece) {
+            ok = mx_wait_warp(&kfull[piece % kPieces], (piece / kPieces) & 1, abort_flag, p.err);
+            if (lane == 0) mbar_arrive(&kempty[piece % kPieces]);
           }
-          if ((t >= kScaleStages &&
-               !__all_sync(0xffffffffu, mx_wait_step(done, t - kScaleStages, abort_flag, p.err))) ||
-              !__all_sync(0xffffffffu, mx_wait_step(kfull, t, abort_flag, p.err))) {
+          t += n;
+          tile = tile + n >= kTiles ? tile + n - kTiles : tile + n;
+          continue;
+        }
+        const uint32_t* ws = nullptr;
+        for (int i = 0; i < n; ++i, ++t) {
+          const int sub = i % per_piece;
+          if (sub == 0) {
+            ws = reinterpret_cast<const uint32_t*>(scale + (piece % kPieces) * kPieceBytes);
+            if (!mx_wait_warp(&kfull[piece % kPieces], (piece / kPieces) & 1, abort_flag, p.err)) {
+              ok = false;
+              break;
+            }
+          }
+          const uint4 a = make_uint4(ws[lane * 4 + sub], ws[(lane + 32) * 4 + sub], ws[(lane + 64) * 4 + sub],
+                                     ws[(lane + 96) * 4 + sub]);
+          // the lo scales are 2^-4 of the hi ones (every byte is at least 4)
+          constexpr uint32_t kLo = 0x04040404u;
+          uint4 b, low;
+          b.x = rs[mine * 4 + i];
+          if (rows == 16) {
+            if (lane >= 16) b.x -= kLo;
+          } else if (rows == 32) {
+            b.y = b.x - kLo;
+          } else {
+            b.y = rs[(lane + 32) * 4 + i];
+            if (rows == 64) {
+              b.z = b.x - kLo;
+              b.w = b.y - kLo;
+            } else {
+              b.z = rs[(lane + 64) * 4 + i];
+              b.w = rs[(lane + 96) * 4 + i];
+              low = make_uint4(b.x - kLo, b.y - kLo, b.z - kLo, b.w - kLo);
+            }
+          }
+          if (t >= kTiles &&
+              !__all_sync(0xffffffffu, mx_wait_step(done, t - kTiles, abort_flag, p.err))) {
             ok = false;
             break;
           }
-          const uint32_t* sa = reinterpret_cast<const uint32_t*>(scale + stage * kScaleBytes) + lane;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) a[c] = sa[32 * c];
-          const uint32_t at = mine + (t % kScaleStages) * 16;
-          tc_fence_after();
-          tmem_st4(at, a);
-          tmem_st4(at + 4, hi);
-          tmem_st4(at + 8, lo);
-          tmem_st_wait();
-          tc_fence_before();
+          uint4* to = reinterpret_cast<uint4*>(tiles + tile * kTileBytes) + lane;
+          to[0] = a;
+          to[32] = b;
+          if (rows == 128) to[64] = low;
+          fence_proxy_async();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&full[t % kBars]);
-          ++t;
-          if (++stage == code_stages) stage = 0;
+          if (lane == 0) {
+            mbar_arrive(&full[t % kBars]);
+            if (sub == per_piece - 1) mbar_arrive(&kempty[piece % kPieces]);
+            if (i == n - 1) mbar_arrive(&bempty[rp]);
+          }
+          piece += sub == per_piece - 1;
+          if (++tile == kTiles) tile = 0;
         }
       }
     }
   } else if (warp == 1) {
     // ---------------- MMA ----------------
     if (elect_one()) {
-      uint32_t t = 0, cstage = 0, rstage = 0;
+      uint32_t t = 0, cstage = 0, rstage = 0, tile = 0;
       int acc = 0;
       uint32_t acc_phase = 0;
       bool ok = true;
       while (ok) {
         if (!mx_wait(&ifull[q], qphase, abort_flag, p.err)) break;
         const int kind = ring[q].phase;
-        const uint32_t n = static_cast<uint32_t>(ring[q].count + 15) & ~15u;
+        const uint32_t rows = mx_rows(ring[q].count);
         mbar_arrive(&iempty[q]);
         if (++q == kRing) { q = 0; qphase ^= 1; }
         if (kind == 0) break;
-        const uint32_t idesc = mx_idesc(n, 0);
+        // up to 64 routes: hi and lo side by side in one MMA of twice the columns
+        // (added up in the epilogue), so that the weights are read once; 128: one
+        // after the other into the same columns
+        const bool wide = rows == 128;
+        const uint32_t idesc = mx_idesc(wide ? 128 : 2 * rows, 0);
         const int steps = (kind == 1 ? p.hidden : p.inter) / kStepK;
         if (!mx_wait(&tempty[acc], acc_phase ^ 1, abort_flag, p.err)) break;
         tc_fence_after();
@@ -538,19 +644,23 @@ __global__ void __launch_bounds__(kMxThreads, 1)
         for (int kb = 0; kb < steps; ++kb, ++t) {
           if (!mx_wait_step(full, t, abort_flag, p.err)) { ok = false; break; }
           tc_fence_after();
-          const uint32_t a = smem_u32(smem + cstage * kCodeBytes);
-          const uint32_t b = smem_u32(routes + rstage * route_bytes);
-          const uint32_t sf = tmem + kTmemScale + (t % kScaleStages) * 16;
+          const uint64_t a = smem_desc_sw128(smem_u32(smem + cstage * kCodeBytes));
+          const uint64_t b = smem_desc_sw128(smem_u32(routes + rstage * route_bytes));
+          const uint32_t sa = tmem + kTmemScale + (t & 3) * 16;
+          const uint32_t from = smem_u32(tiles + tile * kTileBytes);
+          tmem_copy_scales(sa, from);
+          tmem_copy_scales(sa + 4, from + 512);
+          if (wide) tmem_copy_scales(sa + 8, from + 1024);
 #pragma unroll
-          for (uint32_t k = 0; k < 4; ++k) {
+          for (uint32_t k = 0; k < 4; ++k) {  // 32 columns: 32 bytes, 2 in the descriptors' unit
             const uint32_t id = idesc | (k << 4) | (k << 29);
-            const uint64_t ad = smem_desc_sw128(a + k * 32);
-            umma_mxf8f6f4(d, ad, smem_desc_sw128(b + k * 32), id, sf, sf + 4, (kb > 0 || k > 0) ? 1u : 0u);
-            umma_mxf8f6f4(d, ad, smem_desc_sw128(b + route_bytes / 2 + k * 32), id, sf, sf + 8, 1u);
+            umma_mxf8f6f4(d, a + 2 * k, b + 2 * k, id, sa, sa + 4, (kb > 0 || k > 0) ? 1u : 0u);
+            if (wide) umma_mxf8f6f4(d, a + 2 * k, b + 2 * k + (128 * kStepK >> 4), id, sa, sa + 8, 1u);
           }
           umma_commit(&done[t % kBars]);
           if (++cstage == code_stages) cstage = 0;
           if (++rstage == route_stages) rstage = 0;
+          if (++tile == kTiles) tile = 0;
         }
         if (!ok) break;
         umma_commit(&tfull[acc]);
@@ -592,62 +702,75 @@ __global__ void __launch_bounds__(kMxThreads, 1)
       acc_phase ^= 1;
       tc_fence_after();
       const uint32_t d = tmem + (static_cast<uint32_t>(qd * 32) << 16) + eg * kMxN;
+      // 8 columns from c0 on: the hi part's sums, plus the lo part's where they
+      // have columns of their own
+      const int lo_at = it.count > 64 ? 0 : mx_rows(it.count);
+      auto columns = [&](int c0, float* v) {
+        tmem_ld8(d + c0, v);
+        if (lo_at) {
+          float more[8];
+          tmem_ld8(d + lo_at + c0, more);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] += more[j];
+        }
+      };
       if (it.phase == 1) {
-        // 32 routes at a time: gate warps finish the first 16, up warps the rest
+        // 16 routes at a time: gate warps finish the first 8, up warps the rest
         const int block = it.tile * 2 + (qd & 1);  // of 32 features
-        for (int c0 = 0; c0 < it.count; c0 += 32) {
-          float lo[16], hi[16];
-          tmem_ld16(d + c0, lo);
-          tmem_ld16(d + c0 + 16, hi);
+        for (int c0 = 0; c0 < it.count; c0 += 16) {
+          float lo[8], hi[8];
+          columns(c0, lo);
+          columns(c0 + 8, hi);
 #pragma unroll
-          for (int j = 0; j < 16; ++j) give[j] = up_rows ? lo[j] : hi[j];
+          for (int j = 0; j < 8; ++j) give[j] = up_rows ? lo[j] : hi[j];
           mx_epilogue_sync(eg);
-          const int first = c0 + (up_rows ? 16 : 0);
-          uint8_t* to = p.act + static_cast<int64_t>(it.start + first) * (2 * p.inter) + it.tile * kMxFeatures +
-                        f_local;
-          uint8_t* sb = p.as + static_cast<int64_t>(it.start + first) * p.pitch2 + block;
+          const int first = c0 + (up_rows ? 8 : 0);
+          const int n = it.count - first;  // of these 8 routes
+          if (n > 0) {
+            // no branches between the routes: 8 independent chains
+            float a[8];
+            uint32_t top[8], h[4], l[4];
 #pragma unroll
-          for (int j = 0; j < 16; j += 2) {
-            if (first + j < it.count) {  // the same for the whole warp
-              float a[2];
+            for (int j = 0; j < 8; ++j) {
+              const float gate = up_rows ? take[j] : lo[j];
+              const float up = up_rows ? hi[j] : take[j];
+              a[j] = __fdividef(gate, 1.0f + __expf(-gate)) * up;
+            }
 #pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                const float gate = up_rows ? take[j + i] : lo[j + i];
-                const float up = up_rows ? hi[j + i] : take[j + i];
-                a[i] = __fdividef(gate, 1.0f + __expf(-gate)) * up;
-              }
-              int byte[2];
+            for (int j = 0; j < 8; ++j)
+              top[j] = __reduce_max_sync(0xffffffffu, __float_as_uint(a[j]) & 0x7fffffffu);
 #pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(a[i]) & 0x7fffffffu);
-                byte[i] = mx_block_byte(top >> 23);
-                a[i] *= mx_block_mult(byte[i]);
+            for (int j = 0; j < 8; ++j) {
+              top[j] = mx_block_byte(top[j] >> 23);
+              a[j] *= mx_block_mult(top[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) mx_split2(a[2 * j], a[2 * j + 1], &h[j], &l[j]);
+            uint8_t* to = p.act + static_cast<int64_t>(it.start + first) * (2 * p.inter) +
+                          it.tile * kMxFeatures + f_local;
+            uint8_t* sb = p.as + static_cast<int64_t>(it.start + first) * p.pitch2 + block;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              if (j < n) {
+                to[0] = static_cast<uint8_t>(j & 1 ? h[j / 2] >> 8 : h[j / 2]);
+                to[p.inter] = static_cast<uint8_t>(j & 1 ? l[j / 2] >> 8 : l[j / 2]);
+                if (lane == 0) sb[0] = static_cast<uint8_t>(top[j]);
               }
-              uint32_t h, l;
-              mx_split2(a[0], a[1], &h, &l);
-              to[0] = static_cast<uint8_t>(h);
-              to[p.inter] = static_cast<uint8_t>(l);
-              if (lane == 0) sb[0] = static_cast<uint8_t>(byte[0]);
-              if (first + j + 1 < it.count) {
-                to[2 * p.inter] = static_cast<uint8_t>(h >> 8);
-                to[3 * p.inter] = static_cast<uint8_t>(l >> 8);
-                if (lane == 0) sb[p.pitch2] = static_cast<uint8_t>(byte[1]);
-              }
-              to += 4 * p.inter;
-              sb += 2 * p.pitch2;
+              to += 2 * p.inter;
+              sb += p.pitch2;
             }
           }
           mx_epilogue_sync(eg);
         }
       } else {
         __nv_bfloat16* to = p.out + static_cast<int64_t>(it.start) * p.hidden + it.tile * kMxM + qd * 32 + lane;
-        for (int c0 = 0; c0 < it.count; c0 += 16) {
-          float v[16];
-          tmem_ld16(d + c0, v);
+        for (int c0 = 0; c0 < it.count; c0 += 8) {
+          float v[8];
+          columns(c0, v);
           const float ws = c0 < 32 ? w[0] : c0 < 64 ? w[1] : c0 < 96 ? w[2] : w[3];
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float wj = __shfl_sync(0xffffffffu, ws, (c0 & 16) + j);
+          for (int j = 0; j < 8; ++j) {
+            const float wj = __shfl_sync(0xffffffffu, ws, (c0 & 24) + j);
             if (c0 + j < it.count) *to = __float2bfloat16_rn(v[j] * wj);
             to += p.hidden;
           }
@@ -844,17 +967,18 @@ static int make_map_codes(CUtensorMap* map, const void* base, uint64_t cols, uin
   return FERRYB_OK;
 }
 
-// Rows of bytes, boxes of 128 bytes x box_rows.
+// Rows of bytes; boxes 128 bytes wide are swizzled, as the MMA reads them.
 static int make_map_bytes(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols,
-                          uint32_t box_rows) {
+                          uint32_t box_cols, uint32_t box_rows) {
   PFN_encodeTiled enc = encode_tiled_fn();
   if (!enc) return fail(FERRYB_ECUDA, "cuTensorMapEncodeTiled is unavailable");
   cuuint64_t dims[2] = {cols, rows};
   cuuint64_t strides[1] = {cols};
-  cuuint32_t box[2] = {kStepK, box_rows};
+  cuuint32_t box[2] = {box_cols, box_rows};
   cuuint32_t elem[2] = {1, 1};
   CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box,
-                   elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   box_cols == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     return fail(FERRYB_ECUDA, "cuTensorMapEncodeTiled failed (%d) for %llu x %llu bytes", (int)r,
@@ -968,10 +1092,12 @@ extern "C" int ferryb_execute_experts_mxfp4(const ferryb_mxfp4_experts_args* e, 
   if ((s = make_map_codes(&maps.w2, cache + hi, e->intermediate, e->hidden, e->cache_slots, row_bytes,
                           kMxM)))
     return s;
-  if ((s = make_map_bytes(&maps.x16, base + ws.x, e->routes, 2 * e->hidden, 16))) return s;
-  if ((s = make_map_bytes(&maps.x64, base + ws.x, e->routes, 2 * e->hidden, 64))) return s;
-  if ((s = make_map_bytes(&maps.a16, base + ws.act, e->routes, 2 * e->intermediate, 16))) return s;
-  if ((s = make_map_bytes(&maps.a64, base + ws.act, e->routes, 2 * e->intermediate, 64))) return s;
+  if ((s = make_map_bytes(&maps.x16, base + ws.x, e->routes, 2 * e->hidden, kStepK, 16))) return s;
+  if ((s = make_map_bytes(&maps.x64, base + ws.x, e->routes, 2 * e->hidden, kStepK, 64))) return s;
+  if ((s = make_map_bytes(&maps.a16, base + ws.act, e->routes, 2 * e->intermediate, kStepK, 16))) return s;
+  if ((s = make_map_bytes(&maps.a64, base + ws.act, e->routes, 2 * e->intermediate, kStepK, 64))) return s;
+  if ((s = make_map_bytes(&maps.xs, base + ws.xs, e->routes, ws.pitch1, 16, 16))) return s;
+  if ((s = make_map_bytes(&maps.as, base + ws.as, e->routes, ws.pitch2, 16, 16))) return s;
   MxParams p{};
   p.groups = pr.groups;
   p.header = pr.header;
@@ -981,10 +1107,8 @@ extern "C" int ferryb_execute_experts_mxfp4(const ferryb_mxfp4_experts_args* e, 
   p.inter = static_cast<int>(e->intermediate);
   p.scales = cache + 3 * hi / 2;
   p.row_bytes = row_bytes;
-  p.xs = pr.xs;
   p.act = base + ws.act;
   p.as = base + ws.as;
-  p.pitch1 = pr.pitch1;
   p.pitch2 = static_cast<int>(ws.pitch2);
   p.out = static_cast<__nv_bfloat16*>(e->out);
   p.route_w = pr.route_w;
