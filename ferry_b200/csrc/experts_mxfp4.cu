@@ -58,21 +58,21 @@ constexpr int kFirstEpi = 2, kRouteWarp = 10, kFirstScale = 11, kScaleLoad = 15;
 constexpr int kMxM = 128;          // weight rows per tile
 constexpr int kMxN = 128;          // most routes of a sub-group
 constexpr int kStepK = 128;        // columns per step
+constexpr int kSpan = 2;           // steps per load and barrier
 constexpr int kMxFeatures = 64;    // gate (= up) rows per phase-1 tile
-constexpr int kBars = 16;          // barriers of the step pipeline, more than any buffer's depth
+constexpr int kBars = 8;           // barriers of the spans' pipeline, more than any buffer's depth
 constexpr int kBlock = 4;          // steps whose scales come in one piece and are arranged by one warp
-constexpr int kTiles = 6;          // steps whose arranged scales shared memory holds
-constexpr int kPieces = 3;         // pieces of scales in shared memory, weights' and routes'
-constexpr uint32_t kCodeBytes = kMxM * kStepK;  // unpacked
+constexpr int kPieces = 4;         // places for a block's scales as they are in memory
+constexpr uint32_t kStepCodes = kMxM * kStepK;  // a step's codes, unpacked
+constexpr uint32_t kCodeBytes = kSpan * kStepCodes;
 constexpr uint32_t kPieceBytes = kMxM * 16;  // of up to four steps
-constexpr uint32_t kTileBytes = 3 * 512;  // scales of the weights, of the routes, lo scales of 128 routes
+constexpr uint32_t kScalePool = 24 * 1024;  // scales as they are in memory, and arranged
 constexpr uint32_t kTmemScale = 256;  // first TMEM column of the scales: four places of 16 columns
 constexpr int kRing = 4;           // claimed items in flight
 constexpr int kXStride = 9;        // floats a feature of the gate/up exchange (padded)
 constexpr uint32_t kXchgBytes = 2 * kMxFeatures * kXStride * 4;  // an epilogue group's
 constexpr uint32_t kPoolBytes = 12 * 16384;  // codes and routes
-constexpr uint32_t kMxSmem = kPoolBytes + 2 * kPieces * kPieceBytes + kTiles * kTileBytes + 1024 +
-                             1024;
+constexpr uint32_t kMxSmem = kPoolBytes + kScalePool + 1024 + 1024;
 constexpr uint64_t kMxWaitNs = 2000000000ull;  // bound on any wait
 
 // Up to 128 routes of one group.
@@ -94,6 +94,7 @@ struct MxParams {
   const MxGroup* groups;
   MxHeader* header;
   int mt1, mt2;         // items per sub-group: I / 64 phase 1, H / 128 phase 2
+  int tma1, tma2;       // weight scales of phase 1 (2) through s1 (s2): rows of 16-byte multiples
   int hidden, inter;
   const uint8_t* scales;  // slot 0's scale bytes
   int64_t row_bytes;      // bytes of a cache row
@@ -107,10 +108,10 @@ struct MxParams {
 };
 
 struct MxMaps {
-  CUtensorMap w1, w2;        // codes of gate and up rows (64-row boxes), of down rows (128)
-  CUtensorMap x16, x64;      // routes [routes, 2 * H], boxes of 16 and 64 rows
-  CUtensorMap a16, a64;      // activations [routes, 2 * I]
-  CUtensorMap xs, as;        // their scale bytes [routes, pitch], boxes of 16 x 16
+  CUtensorMap w1, w2;      // codes of gate and up rows, of down rows
+  CUtensorMap x[4], a[4];  // routes and activations, 16, 32, 64, 128 rows at once
+  CUtensorMap xs, as;      // their scale bytes [routes, pitch], 16 rows x 16 bytes at once
+  CUtensorMap s1, s2;      // scale bytes of gate and up rows, of down rows, 16 bytes of 128 rows
 };
 
 // A claimed work item, handed from warp 0 to the other roles.
@@ -179,12 +180,29 @@ __device__ __forceinline__ bool mx_wait_warp(uint64_t* bar, uint32_t parity,
   return __all_sync(0xffffffffu, mx_wait(bar, parity, abort_flag, err));
 }
 
-__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar,
-                                            int32_t x, int32_t y, int32_t z) {
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int32_t c0,
+                                            int32_t c1, int32_t c2) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
       " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int32_t c0,
+                                            int32_t c1, int32_t c2, int32_t c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, uint64_t* bar, int32_t c0,
+                                            int32_t c1, int32_t c2, int32_t c3, int32_t c4) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3),
+      "r"(c4)
       : "memory");
 }
 template <int BYTES>
@@ -200,12 +218,13 @@ __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
 
 // 32 rows of 16 bytes of shared memory (rows one after the other) into 4 columns
 // of every 32-lane quarter of tensor memory.  Ordered before the MMAs that the
-// same thread issues after it.
-__device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint32_t saddr) {
-  // descriptor: address >> 4, 8-row groups 128 bytes apart (bits 32-45), version
-  // 1 (bits 46-47), no swizzle
-  const uint64_t desc = static_cast<uint64_t>((saddr >> 4) & 0x3FFF) | (static_cast<uint64_t>(1) << 16) |
-                        (static_cast<uint64_t>(128 >> 4) << 32) | (static_cast<uint64_t>(1) << 46);
+// same thread issues after it.  Descriptor: address >> 4, 8-row groups 128 bytes
+// apart (bits 32-45), version 1 (bits 46-47), no swizzle.
+__device__ __forceinline__ uint64_t smem_desc_scales(uint32_t saddr) {
+  return static_cast<uint64_t>((saddr >> 4) & 0x3FFF) | (static_cast<uint64_t>(1) << 16) |
+         (static_cast<uint64_t>(128 >> 4) << 32) | (static_cast<uint64_t>(1) << 46);
+}
+__device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint64_t desc) {
   asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
 // 32 lanes x 8 consecutive columns of 32 bits.
@@ -239,6 +258,24 @@ __device__ __forceinline__ void umma_mxf8f6f4(uint32_t tmem_d, uint64_t adesc, u
 // bits 4-5 for B and 29-30 for A.
 __device__ __forceinline__ uint32_t mx_idesc(uint32_t n, uint32_t byte) {
   return (5u << 7) | ((n >> 3) << 17) | (1u << 23) | (1u << 27) | (byte << 4) | (byte << 29);
+}
+
+// A step: its scales into tensor memory, then four K = 32 MMAs (eight with WIDE:
+// hi, then lo into the same columns).  Descriptors count in 16 bytes: 32 columns
+// are 2, 512 bytes of scales 32, the 128 rows of a wide hi part 1024.
+template <bool WIDE>
+__device__ __forceinline__ void issue_step(uint32_t d, uint64_t a, uint64_t b, uint32_t b_off, uint32_t sa,
+                                           uint64_t from, uint32_t idesc, bool accumulate) {
+  tmem_copy_scales(sa, from);
+  tmem_copy_scales(sa + 4, from + 32);
+  if (WIDE) tmem_copy_scales(sa + 8, from + 64);
+  b += b_off;
+#pragma unroll
+  for (uint32_t k = 0; k < 4; ++k) {
+    const uint32_t id = idesc | (k << 4) | (k << 29);
+    umma_mxf8f6f4(d, a + 2 * k, b + 2 * k, id, sa, sa + 4, accumulate || k > 0 ? 1u : 0u);
+    if (WIDE) umma_mxf8f6f4(d, a + 2 * k, b + 1024 + 2 * k, id, sa, sa + 8, 1u);
+  }
 }
 
 // ---- hi and lo parts of values ----
@@ -280,33 +317,37 @@ __device__ __forceinline__ bool mx_epilogue_all(int g, bool v) {
   return r != 0;
 }
 
-// The pool of shared memory, by the sub-groups' size: stages of codes first,
-// then stages of routes (hi and lo parts of `box` rows).  Deep code rings where
-// routes are few (memory-bound), enough of both where they are many.
+// The pool of shared memory, by the sub-groups' size: places of codes first, then
+// places of routes (hi and lo parts of `box` rows), a span each.  Many places
+// for codes where routes are few (memory-bound), as many of both where they
+// are many.
 __host__ __device__ __forceinline__ int mx_code_stages(int box) {
-  return box == 0 ? 10 : box == 1 ? 9 : box == 2 ? 8 : 4;
+  return box == 0 ? 5 : box == 1 ? 4 : box == 2 ? 3 : 2;
 }
 __host__ __device__ __forceinline__ int mx_route_stages(int box) {
-  return box == 0 ? 8 : box == 1 ? 6 : 4;
+  return box == 0 ? 4 : box == 1 ? 4 : box == 2 ? 3 : 2;
 }
-__host__ __device__ __forceinline__ uint32_t mx_route_bytes(int box) { return (16u << box) * kStepK * 2; }
+__host__ __device__ __forceinline__ uint32_t mx_route_bytes(int box) {
+  return (16u << box) * kStepK * 2 * kSpan;
+}
 
 // Rows of routes that a sub-group's tile holds: 16, 32, 64 or 128.
-__device__ __forceinline__ int mx_rows(int count) {
-  return count <= 16 ? 16 : count <= 32 ? 32 : count <= 64 ? 64 : 128;
+__device__ __forceinline__ int mx_class(int count) {
+  return count <= 16 ? 0 : count <= 32 ? 1 : count <= 64 ? 2 : 3;
 }
+__device__ __forceinline__ int mx_rows(int count) { return 16 << mx_class(count); }
 
-// Steps are numbered from 0 over all items of a CTA.  Step t uses barrier t % 16
-// of each pipeline; a buffer of S stages may be refilled for step t once step
-// t - S is done, and S < 16 keeps the parity unambiguous.
-__device__ __forceinline__ bool mx_wait_step(uint64_t* bars, uint32_t t, volatile int* abort_flag,
+// A span is two steps: loads, barriers and commits cost the one thread that
+// issues them 100 to 300 cycles each (a TMA load alone 290, the next one behind
+// it 50), which by the step was more than the step's 375 cycles of HBM time.
+// Spans are numbered from 0 over all items of a CTA (an item's last span may be
+// half empty: zeros).  Span t uses barrier t % 8 of each pipeline; a buffer of S
+// places may be refilled for span t once span t - S is done, and S < 8 keeps the
+// parity unambiguous.
+__device__ __forceinline__ bool mx_wait_span(uint64_t* bars, uint32_t t, volatile int* abort_flag,
                                              int* err) {
   return mx_wait(bars + t % kBars, (t / kBars) & 1, abort_flag, err);
 }
-
-// Scale bytes of a row that are copied at once (16, 8 or 4): rows of K / 32 bytes
-// start on multiples of the widest of them that divides the row.
-__device__ __forceinline__ int mx_piece(int K) { return K % 512 == 0 ? 16 : K % 256 == 0 ? 8 : 4; }
 
 // Wait until the sub-group's activations are written: four epilogue warps for
 // each of its phase-1 tiles.
@@ -332,16 +373,12 @@ __global__ void __launch_bounds__(kMxThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
-  uint8_t* scale = smem + kPoolBytes;  // [pieces][128 rows] 16 scale bytes
-  uint8_t* rscale = scale + kPieces * kPieceBytes;  // the same of the routes
-  uint8_t* tiles = rscale + kPieces * kPieceBytes;  // [kTiles] arranged scales
-  uint64_t* full = reinterpret_cast<uint64_t*>(tiles + kTiles * kTileBytes);
+  uint8_t* scale = smem + kPoolBytes;  // places of weights' scales [128 rows] 16 bytes
+  uint64_t* full = reinterpret_cast<uint64_t*>(scale + kScalePool);
   uint64_t* done = full + kBars;     // the MMAs of a step are complete
-  uint64_t* kfull = done + kBars;    // [kPieces] weight scales landed
+  uint64_t* kfull = done + kBars;    // [kPieces] a block's scales landed
   uint64_t* kempty = kfull + kPieces;
-  uint64_t* bfull = kempty + kPieces;  // [kPieces] route scales landed
-  uint64_t* bempty = bfull + kPieces;
-  uint64_t* tfull = bempty + kPieces;  // [2] accumulators
+  uint64_t* tfull = kempty + kPieces;  // [2] accumulators
   uint64_t* tempty = tfull + 2;
   uint64_t* ifull = tempty + 2;      // [kRing] claimed items
   uint64_t* iempty = ifull + kRing;
@@ -358,13 +395,11 @@ __global__ void __launch_bounds__(kMxThreads, 1)
       mbar_init(&done[s], 1);
     }
     for (int s = 0; s < kPieces; ++s) {
-      mbar_init(&kfull[s], 32);
-      mbar_init(&kempty[s], 4);
-      mbar_init(&bfull[s], 1);
-      mbar_init(&bempty[s], 4);
+      mbar_init(&kfull[s], 33);  // TMA, and the lanes' cp.async
+      mbar_init(&kempty[s], 1);
     }
     for (int b = 0; b < 2; ++b) { mbar_init(&tfull[b], 1); mbar_init(&tempty[b], 4); }
-    for (int q = 0; q < kRing; ++q) { mbar_init(&ifull[q], 1); mbar_init(&iempty[q], 15); }
+    for (int q = 0; q < kRing; ++q) { mbar_init(&ifull[q], 1); mbar_init(&iempty[q], 11 + (p.header->box == 3 ? 2 : 4)); }
     mbar_init(drain, 1);
     *abort_flag = 0;
     fence_barrier_init();
@@ -378,6 +413,15 @@ __global__ void __launch_bounds__(kMxThreads, 1)
   const uint32_t code_stages = mx_code_stages(box), route_stages = mx_route_stages(box);
   const uint32_t route_bytes = mx_route_bytes(box);
   uint8_t* const routes = smem + code_stages * kCodeBytes;
+  // Blocks go around the scale warps, each of which has a place of its own for
+  // the weights' and for the routes' bytes.  Arranged, a step has 512 bytes of
+  // weights' scales, 512 of routes' and, for 128 routes, 512 of lo scales: more,
+  // and two warps (and places) instead of four.
+  const uint32_t places = box == 3 ? 2 : 4, tile_bytes = box == 3 ? 1536 : 1024;
+  const uint32_t place_bytes = box == 3 ? kPieceBytes : kPieceBytes / 2;  // of the routes
+  uint8_t* const rscale = scale + places * kPieceBytes;
+  uint8_t* const tiles = rscale + places * place_bytes;
+  const uint32_t tile_spans = box == 3 ? 5 : 6;
   int q = 0;            // this role's place in the item ring
   uint32_t qphase = 0;
 
@@ -397,29 +441,25 @@ __global__ void __launch_bounds__(kMxThreads, 1)
       MxItem it = mx_item(p, n_groups, atomicAdd(&p.header->queue, 1));
       ok = publish(it);
       while (ok && it.phase != 0) {
-        // the next item is claimed now and published a few steps on, before this
-        // one's last loads: its scales and routes are under way in time
+        // the next item is claimed now and published a few loads on, before this
+        // one's last: its scales and routes are under way in time
         const int id = atomicAdd(&p.header->queue, 1);
         MxItem next{};
         const int K = it.phase == 1 ? p.hidden : p.inter;
         const int row0 = it.tile * (it.phase == 1 ? kMxFeatures : kMxM);
-        const int ahead = min(K - kStepK, 3 * kStepK);
-        for (int k0 = 0; k0 < K; k0 += kStepK, ++t) {
-          if (t >= code_stages && !mx_wait_step(done, t - code_stages, abort_flag, p.err)) {
+        const int steps = K / kStepK, ahead = steps > kSpan ? kSpan : 0;
+        for (int kb = 0; kb < steps; kb += kSpan, ++t) {
+          if (t >= code_stages && !mx_wait_span(done, t - code_stages, abort_flag, p.err)) {
             ok = false;
             break;
           }
           uint64_t* bar = full + t % kBars;
           uint8_t* cs = smem + stage * kCodeBytes;
           mbar_expect_tx(bar, kCodeBytes / 2);  // the copy counts its 4-bit data, not the gaps
-          if (it.phase == 1) {
-            tma_load_3d(cs, &maps.w1, bar, k0, row0, it.slot);
-            tma_load_3d(cs + kCodeBytes / 2, &maps.w1, bar, k0, p.inter + row0, it.slot);
-          } else {
-            tma_load_3d(cs, &maps.w2, bar, k0, row0, it.slot);
-          }
+          if (it.phase == 1) tma_load_5d(cs, &maps.w1, bar, 0, row0, 0, kb, it.slot);
+          else tma_load_4d(cs, &maps.w2, bar, 0, row0, kb, it.slot);
           if (++stage == code_stages) stage = 0;
-          if (k0 == ahead) {
+          if (kb == ahead) {
             next = mx_item(p, n_groups, id);
             if (!publish(next)) { ok = false; break; }
           }
@@ -435,55 +475,75 @@ __global__ void __launch_bounds__(kMxThreads, 1)
       }
     }
   } else if (warp == kScaleLoad) {
-    // ---------------- weight scales into shared memory ----------------
-    int piece = 0;
-    uint32_t pphase = 0;
+    // ---------------- scales into shared memory ----------------
+    // Its own warp: the scales of a block go through more hands than the codes
+    // and routes of its steps, and start their way earlier.
+    uint32_t place = 0, ph = 0;
     bool ok = true;
     while (ok) {
       if (!mx_wait_warp(&ifull[q], qphase, abort_flag, p.err)) break;
-      const int phase = ring[q].phase, tile = ring[q].tile, slot = ring[q].slot;
+      const int phase = ring[q].phase, tile = ring[q].tile, slot = ring[q].slot, group = ring[q].group;
+      const int start = ring[q].start, rows = mx_rows(ring[q].count);
       __syncwarp();
       if (lane == 0) mbar_arrive(&iempty[q]);
       if (++q == kRing) { q = 0; qphase ^= 1; }
       if (phase == 0) break;
       const int K = phase == 1 ? p.hidden : p.inter;
-      // tile rows lane + 32 * i, a piece of 4, 2 or 1 steps (the widest copy
-      // that the rows' alignment allows) each
-      const int pitch = K / 32, width = mx_piece(K);
+      // 16 bytes (four steps) of each tile row: one TMA load where the rows are
+      // 16-byte multiples (K a multiple of 512), else cp.async of 8 or 4 bytes, rows
+      // lane + 32 * i
+      const bool tma = (phase == 1 ? p.tma1 : p.tma2) != 0;
+      const int pitch = K / 32;
       const uint8_t* src = p.scales + slot * p.row_bytes +
                            (phase == 1 ? 0 : 2 * static_cast<int64_t>(p.inter) * (p.hidden / 32)) +
                            static_cast<int64_t>(tile * (phase == 1 ? kMxFeatures : kMxM) + lane) * pitch;
       const int64_t d1 = 32 * pitch;
       const int64_t d2 = phase == 1 ? static_cast<int64_t>(p.inter) * pitch : 2 * d1;  // up rows
-      for (int b = 0; b < pitch; b += width) {
-        if (!mx_wait_warp(&kempty[piece], pphase ^ 1, abort_flag, p.err)) { ok = false; break; }
-        uint8_t* to = scale + piece * kPieceBytes + lane * 16;
-        if (width == 16) {
-          cp_async<16>(to, src + b);
-          cp_async<16>(to + 512, src + b + d1);
-          cp_async<16>(to + 1024, src + b + d2);
-          cp_async<16>(to + 1536, src + b + d2 + d1);
-        } else if (width == 8) {
-          cp_async<8>(to, src + b);
-          cp_async<8>(to + 512, src + b + d1);
-          cp_async<8>(to + 1024, src + b + d2);
-          cp_async<8>(to + 1536, src + b + d2 + d1);
-        } else {
-          cp_async<4>(to, src + b);
-          cp_async<4>(to + 512, src + b + d1);
-          cp_async<4>(to + 1024, src + b + d2);
-          cp_async<4>(to + 1536, src + b + d2 + d1);
+      if (phase == 2) {
+        bool there = true;
+        if (lane == 0) there = mx_wait_dep(p.dep + group, 4 * p.mt1, abort_flag, p.err);
+        if (!__shfl_sync(0xffffffffu, there, 0)) break;
+        asm volatile("fence.proxy.async.global;" ::: "memory");
+      }
+      for (int b = 0; b < pitch; b += 16) {
+        if (!mx_wait_warp(&kempty[place], ph ^ 1, abort_flag, p.err)) { ok = false; break; }
+        uint8_t* to = scale + place * kPieceBytes;
+        if (lane == 0) {
+          mbar_expect_tx(&kfull[place], rows * 16 + (tma ? kPieceBytes : 0));
+          if (tma && phase == 1) tma_load_4d(to, &maps.s1, &kfull[place], b, tile * kMxFeatures, 0, slot);
+          else if (tma) tma_load_3d(to, &maps.s2, &kfull[place], b, tile * kMxM, slot);
+          for (int i = 0; i < rows; i += 16)
+            tma_load_2d(rscale + place * place_bytes + i * 16, phase == 1 ? &maps.xs : &maps.as, &kfull[place], b,
+                        start + i);
         }
-        cp_async_arrive(&kfull[piece]);
-        if (++piece == kPieces) { piece = 0; pphase ^= 1; }
+        __syncwarp();
+        to += lane * 16;
+        const uint8_t* from = src + b;
+        if (tma) {
+        } else if (pitch % 8 == 0) {
+          for (int i = 0; i < min(16, pitch - b); i += 8) {
+            cp_async<8>(to + i, from + i);
+            cp_async<8>(to + 512 + i, from + d1 + i);
+            cp_async<8>(to + 1024 + i, from + d2 + i);
+            cp_async<8>(to + 1536 + i, from + d2 + d1 + i);
+          }
+        } else {
+          for (int i = 0; i < min(16, pitch - b); i += 4) {
+            cp_async<4>(to + i, from + i);
+            cp_async<4>(to + 512 + i, from + d1 + i);
+            cp_async<4>(to + 1024 + i, from + d2 + i);
+            cp_async<4>(to + 1536 + i, from + d2 + d1 + i);
+          }
+        }
+        cp_async_arrive(&kfull[place]);
+        if (++place == places) { place = 0; ph ^= 1; }
       }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp == kRouteWarp) {
     // ---------------- routes ----------------
     if (elect_one()) {
-      uint32_t t = 0, stage = 0, bphase = 0;
-      int piece = 0;
+      uint32_t t = 0, stage = 0;
       bool ok = true;
       while (ok) {
         if (!mx_wait(&ifull[q], qphase, abort_flag, p.err)) { ok = false; break; }
@@ -495,34 +555,18 @@ __global__ void __launch_bounds__(kMxThreads, 1)
           if (!mx_wait_dep(p.dep + it.group, 4 * p.mt1, abort_flag, p.err)) { ok = false; break; }
           asm volatile("fence.proxy.async.global;" ::: "memory");
         }
-        const int K = it.phase == 1 ? p.hidden : p.inter;
-        // 16 or 32 rows in boxes of 16, 64 or 128 in boxes of 64; the lo part's
-        // rows follow the hi part's
-        const int n = mx_rows(it.count);
-        const int rows = n <= 32 ? 16 : 64;
-        const int boxes = n / rows;
-        const CUtensorMap* map = it.phase == 1 ? (rows == 16 ? &maps.x16 : &maps.x64)
-                                               : (rows == 16 ? &maps.a16 : &maps.a64);
-        const CUtensorMap* smap = it.phase == 1 ? &maps.xs : &maps.as;
-        for (int k0 = 0; k0 < K; k0 += kStepK, ++t) {
-          if (k0 % (kBlock * kStepK) == 0) {  // the scale bytes of four steps
-            if (!mx_wait(&bempty[piece], bphase ^ 1, abort_flag, p.err)) { ok = false; break; }
-            mbar_expect_tx(&bfull[piece], n * 16);
-            for (int i = 0; i < n; i += 16)
-              tma_load_2d(rscale + piece * kPieceBytes + i * 16, smap, &bfull[piece], k0 / 32, it.start + i);
-            if (++piece == kPieces) { piece = 0; bphase ^= 1; }
-          }
-          if (t >= route_stages && !mx_wait_step(done, t - route_stages, abort_flag, p.err)) {
+        const int steps = (it.phase == 1 ? p.hidden : p.inter) / kStepK;
+        const int cls = mx_class(it.count);
+        const CUtensorMap* map = it.phase == 1 ? &maps.x[cls] : &maps.a[cls];
+        for (int kb = 0; kb < steps; kb += kSpan, ++t) {
+          if (t >= route_stages && !mx_wait_span(done, t - route_stages, abort_flag, p.err)) {
             ok = false;
             break;
           }
           uint64_t* bar = full + t % kBars;
-          uint8_t* to = routes + stage * route_bytes;
-          mbar_expect_tx(bar, static_cast<uint32_t>(boxes * rows * kStepK * 2));
-          for (int i = 0; i < boxes; ++i) {
-            tma_load_2d(to + i * rows * kStepK, map, bar, k0, it.start + i * rows);
-            tma_load_2d(to + (n + i * rows) * kStepK, map, bar, K + k0, it.start + i * rows);
-          }
+          mbar_expect_tx(bar, (16u << cls) * kStepK * 2 * kSpan);
+          // per step the rows' hi parts, then their lo parts
+          tma_load_4d(routes + stage * route_bytes, map, bar, 0, it.start, 0, kb);
           if (++stage == route_stages) stage = 0;
         }
       }
@@ -535,93 +579,80 @@ __global__ void __launch_bounds__(kMxThreads, 1)
   } else if (warp >= kFirstScale) {
     // ---------------- scales arranged ----------------
     // Into the MMA's order: row r's four bytes of a step at (r % 32) * 16 + r / 32
-    // * 4.  A block of up to four steps is one warp's, the blocks go around.  All
-    // four warps wait for and release every piece, so that none falls behind a
-    // barrier by more than a phase.
-    uint32_t t = 0, blk = 0, piece = 0, tile = 0;  // counted over all items
-    bool ok = true;
+    // * 4.
+    const uint32_t me = warp - kFirstScale;
+    uint32_t t = 0, turn = 0, ph = 0;  // spans and blocks of all items
+    bool ok = me < places;
     while (ok) {
       if (!mx_wait_warp(&ifull[q], qphase, abort_flag, p.err)) break;
-      const int phase = ring[q].phase, count = ring[q].count;
+      const int phase = ring[q].phase, rows = mx_rows(ring[q].count);
       __syncwarp();
       if (lane == 0) mbar_arrive(&iempty[q]);
       if (++q == kRing) { q = 0; qphase ^= 1; }
       if (phase == 0) break;
-      const int K = phase == 1 ? p.hidden : p.inter;
-      const int per_piece = mx_piece(K) / 4;  // steps
-      const int rows = mx_rows(count);
-      const int mine = rows == 16 ? lane & 15 : lane;
-      for (int k0 = 0; k0 < K && ok; k0 += kBlock * kStepK, ++blk) {
-        const int n = min(kBlock, (K - k0) / kStepK);
-        const uint32_t rp = blk % kPieces;
-        const uint32_t* rs = reinterpret_cast<const uint32_t*>(rscale + rp * kPieceBytes);
-        if (!mx_wait_warp(&bfull[rp], (blk / kPieces) & 1, abort_flag, p.err)) { ok = false; break; }
-        if ((blk & 3) != static_cast<uint32_t>(warp - kFirstScale)) {
-          if (lane == 0) mbar_arrive(&bempty[rp]);
-          for (int i = 0; i < n && ok; i += per_piece, ++piece) {
-            ok = mx_wait_warp(&kfull[piece % kPieces], (piece / kPieces) & 1, abort_flag, p.err);
-            if (lane == 0) mbar_arrive(&kempty[piece % kPieces]);
-          }
-          t += n;
-          tile = tile + n >= kTiles ? tile + n - kTiles : tile + n;
-          continue;
+      const int steps = (phase == 1 ? p.hidden : p.inter) / kStepK;
+      for (int k = 0; k < steps; k += kBlock) {
+        const int n = min(kBlock, steps - k);
+        const uint32_t spans = (n + kSpan - 1) / kSpan;
+        const bool mine = turn == me;
+        if (++turn == places) turn = 0;
+        if (!mine) { t += spans; continue; }
+        if (!mx_wait_warp(&kfull[me], ph, abort_flag, p.err)) { ok = false; break; }
+        ph ^= 1;
+        // four steps of weight rows lane + 32 * c, and of routes
+        const uint4* rs = reinterpret_cast<const uint4*>(rscale + me * place_bytes);
+        const uint4* ws = reinterpret_cast<const uint4*>(scale + me * kPieceBytes);
+        uint4 b4[4], a4[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          a4[c] = ws[lane + 32 * c];
+          b4[c] = make_uint4(0, 0, 0, 0);
+          if (c == 0) b4[c] = rs[rows == 16 ? lane & 15 : lane];
+          else if (rows > 32 * c) b4[c] = rs[lane + 32 * c];
         }
-        const uint32_t* ws = nullptr;
-        for (int i = 0; i < n; ++i, ++t) {
-          const int sub = i % per_piece;
-          if (sub == 0) {
-            ws = reinterpret_cast<const uint32_t*>(scale + (piece % kPieces) * kPieceBytes);
-            if (!mx_wait_warp(&kfull[piece % kPieces], (piece / kPieces) & 1, abort_flag, p.err)) {
-              ok = false;
-              break;
-            }
-          }
-          const uint4 a = make_uint4(ws[lane * 4 + sub], ws[(lane + 32) * 4 + sub], ws[(lane + 64) * 4 + sub],
-                                     ws[(lane + 96) * 4 + sub]);
-          // the lo scales are 2^-4 of the hi ones (every byte is at least 4)
-          constexpr uint32_t kLo = 0x04040404u;
-          uint4 b, low;
-          b.x = rs[mine * 4 + i];
-          if (rows == 16) {
-            if (lane >= 16) b.x -= kLo;
-          } else if (rows == 32) {
-            b.y = b.x - kLo;
-          } else {
-            b.y = rs[(lane + 32) * 4 + i];
-            if (rows == 64) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&kempty[me]);
+        // the tiles' last users are done
+        if (t + spans > tile_spans &&
+            !__all_sync(0xffffffffu, mx_wait_span(done, t + spans - 1 - tile_spans, abort_flag, p.err))) {
+          ok = false;
+          break;
+        }
+#pragma unroll
+        for (int i = 0; i < kBlock; ++i) {
+          if (i < n) {
+            auto part = [&](const uint4& v) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; };
+            // the lo scales are 2^-4 of the hi ones (every byte is at least 4)
+            constexpr uint32_t kLo = 0x04040404u;
+            uint4 b = make_uint4(part(b4[0]), part(b4[1]), part(b4[2]), part(b4[3]));
+            uint4* to = reinterpret_cast<uint4*>(
+                            tiles + (((t + i / kSpan) % tile_spans) * kSpan + i % kSpan) * tile_bytes) + lane;
+            if (rows == 16) {
+              if (lane >= 16) b.x -= kLo;
+            } else if (rows == 32) {
+              b.y = b.x - kLo;
+            } else if (rows == 64) {
               b.z = b.x - kLo;
               b.w = b.y - kLo;
             } else {
-              b.z = rs[(lane + 64) * 4 + i];
-              b.w = rs[(lane + 96) * 4 + i];
-              low = make_uint4(b.x - kLo, b.y - kLo, b.z - kLo, b.w - kLo);
+              to[64] = make_uint4(b.x - kLo, b.y - kLo, b.z - kLo, b.w - kLo);
             }
+            to[0] = make_uint4(part(a4[0]), part(a4[1]), part(a4[2]), part(a4[3]));
+            to[32] = b;
           }
-          if (t >= kTiles &&
-              !__all_sync(0xffffffffu, mx_wait_step(done, t - kTiles, abort_flag, p.err))) {
-            ok = false;
-            break;
-          }
-          uint4* to = reinterpret_cast<uint4*>(tiles + tile * kTileBytes) + lane;
-          to[0] = a;
-          to[32] = b;
-          if (rows == 128) to[64] = low;
-          fence_proxy_async();
-          __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(&full[t % kBars]);
-            if (sub == per_piece - 1) mbar_arrive(&kempty[piece % kPieces]);
-            if (i == n - 1) mbar_arrive(&bempty[rp]);
-          }
-          piece += sub == per_piece - 1;
-          if (++tile == kTiles) tile = 0;
         }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane < static_cast<int>(spans)) mbar_arrive(&full[(t + lane) % kBars]);
+        t += spans;
       }
     }
   } else if (warp == 1) {
     // ---------------- MMA ----------------
     if (elect_one()) {
-      uint32_t t = 0, cstage = 0, rstage = 0, tile = 0;
+      uint32_t t = 0, cstage = 0, rstage = 0, tspan = 0;
+      const uint64_t a0 = smem_desc_sw128(smem_u32(smem)), b0 = smem_desc_sw128(smem_u32(routes));
+      const uint64_t s0 = smem_desc_scales(smem_u32(tiles));
       int acc = 0;
       uint32_t acc_phase = 0;
       bool ok = true;
@@ -641,26 +672,26 @@ __global__ void __launch_bounds__(kMxThreads, 1)
         if (!mx_wait(&tempty[acc], acc_phase ^ 1, abort_flag, p.err)) break;
         tc_fence_after();
         const uint32_t d = tmem + acc * kMxN;
-        for (int kb = 0; kb < steps; ++kb, ++t) {
-          if (!mx_wait_step(full, t, abort_flag, p.err)) { ok = false; break; }
+        for (int kb = 0; kb < steps; kb += kSpan, ++t) {
+          if (!mx_wait_span(full, t, abort_flag, p.err)) { ok = false; break; }
           tc_fence_after();
-          const uint64_t a = smem_desc_sw128(smem_u32(smem + cstage * kCodeBytes));
-          const uint64_t b = smem_desc_sw128(smem_u32(routes + rstage * route_bytes));
-          const uint32_t sa = tmem + kTmemScale + (t & 3) * 16;
-          const uint32_t from = smem_u32(tiles + tile * kTileBytes);
-          tmem_copy_scales(sa, from);
-          tmem_copy_scales(sa + 4, from + 512);
-          if (wide) tmem_copy_scales(sa + 8, from + 1024);
-#pragma unroll
-          for (uint32_t k = 0; k < 4; ++k) {  // 32 columns: 32 bytes, 2 in the descriptors' unit
-            const uint32_t id = idesc | (k << 4) | (k << 29);
-            umma_mxf8f6f4(d, a + 2 * k, b + 2 * k, id, sa, sa + 4, (kb > 0 || k > 0) ? 1u : 0u);
-            if (wide) umma_mxf8f6f4(d, a + 2 * k, b + 2 * k + (128 * kStepK >> 4), id, sa, sa + 8, 1u);
+          const uint64_t a = a0 + cstage * (kCodeBytes >> 4), b = b0 + rstage * (route_bytes >> 4);
+          const uint32_t sa = tmem + kTmemScale + (t & 1) * (kSpan * 16);
+          const uint64_t from = s0 + tspan * (kSpan * tile_bytes >> 4);
+          if (wide) {
+            issue_step<true>(d, a, b, 0, sa, from, idesc, kb > 0);
+            if (kb + 1 < steps)
+              issue_step<true>(d, a + (kStepCodes >> 4), b, 256 * kStepK >> 4, sa + 16, from + (1536 >> 4), idesc, true);
+          } else {
+            issue_step<false>(d, a, b, 0, sa, from, idesc, kb > 0);
+            if (kb + 1 < steps)
+              issue_step<false>(d, a + (kStepCodes >> 4), b, rows * (2 * kStepK >> 4), sa + 16, from + (tile_bytes >> 4),
+                                idesc, true);
           }
           umma_commit(&done[t % kBars]);
           if (++cstage == code_stages) cstage = 0;
           if (++rstage == route_stages) rstage = 0;
-          if (++tile == kTiles) tile = 0;
+          if (++tspan == tile_spans) tspan = 0;
         }
         if (!ok) break;
         umma_commit(&tfull[acc]);
@@ -948,41 +979,74 @@ __global__ void __launch_bounds__(kPrepThreads) mxfp4_prepare_kernel(const MxPre
 
 // ---------------------------------------------------------------------------
 // Host side
-// Codes of a weight matrix in every slot: [slots, rows, cols] 4-bit elements,
-// unpacked on the way (16 codes to 16 bytes of shared memory, 8 of them data).
-static int make_map_codes(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows,
-                          uint64_t slots, uint64_t slot_bytes, uint32_t box_rows) {
+static int make_map(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base,
+                    const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box, bool swizzle) {
   PFN_encodeTiled enc = encode_tiled_fn();
   if (!enc) return fail(FERRYB_ECUDA, "cuTensorMapEncodeTiled is unavailable");
-  cuuint64_t dims[3] = {cols, rows, slots};
-  cuuint64_t strides[2] = {cols / 2, slot_bytes};
-  cuuint32_t box[3] = {kStepK, box_rows, 1};
-  cuuint32_t elem[3] = {1, 1, 1};
-  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, 3, const_cast<void*>(base), dims, strides,
-                   box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+  cuuint32_t elem[5] = {1, 1, 1, 1, 1};
+  CUresult r = enc(map, type, rank, const_cast<void*>(base), dims, strides, box, elem,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS)
-    return fail(FERRYB_ECUDA, "cuTensorMapEncodeTiled failed (%d) for %llu x %llu codes", (int)r,
-                (unsigned long long)rows, (unsigned long long)cols);
+  if (r != CUDA_SUCCESS) return fail(FERRYB_ECUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
   return FERRYB_OK;
 }
 
-// Rows of bytes; boxes 128 bytes wide are swizzled, as the MMA reads them.
-static int make_map_bytes(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols,
-                          uint32_t box_cols, uint32_t box_rows) {
-  PFN_encodeTiled enc = encode_tiled_fn();
-  if (!enc) return fail(FERRYB_ECUDA, "cuTensorMapEncodeTiled is unavailable");
-  cuuint64_t dims[2] = {cols, rows};
-  cuuint64_t strides[1] = {cols};
-  cuuint32_t box[2] = {box_cols, box_rows};
-  cuuint32_t elem[2] = {1, 1};
-  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box,
-                   elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   box_cols == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
-                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS)
-    return fail(FERRYB_ECUDA, "cuTensorMapEncodeTiled failed (%d) for %llu x %llu bytes", (int)r,
-                (unsigned long long)rows, (unsigned long long)cols);
+// All maps of a call.  Codes are 4-bit elements, unpacked on the way (16 codes
+// to 16 bytes of shared memory, 8 of them data).  A column index is split into
+// steps of 128 and the column inside, so that one load brings a span: for
+// each of its steps the tile's rows (gate rows, then up rows; for routes the hi
+// parts, then the lo parts), 128 columns each.
+static int make_maps(MxMaps* m, const ferryb_mxfp4_experts_args* e, const uint8_t* x, const uint8_t* act,
+                     const uint8_t* xs, const uint8_t* as, int64_t pitch1, int64_t pitch2) {
+  const cuuint64_t H = e->hidden, I = e->intermediate, slots = e->cache_slots, routes = e->routes;
+  const cuuint64_t row_bytes = 3 * H * I / 32 * 17;
+  const uint8_t* cache = static_cast<const uint8_t*>(e->cache);
+  constexpr auto k4 = CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B;
+  constexpr auto k8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  int s;
+  {
+    const cuuint64_t dims[5] = {kStepK, I, 2, H / kStepK, slots};
+    const cuuint64_t strides[4] = {H / 2, I * H / 2, kStepK / 2, row_bytes};
+    const cuuint32_t box[5] = {kStepK, kMxFeatures, 2, kSpan, 1};
+    if ((s = make_map(&m->w1, k4, 5, cache, dims, strides, box, true))) return s;
+  }
+  {
+    const cuuint64_t dims[4] = {kStepK, H, I / kStepK, slots};
+    const cuuint64_t strides[3] = {I / 2, kStepK / 2, row_bytes};
+    const cuuint32_t box[4] = {kStepK, kMxM, kSpan, 1};
+    if ((s = make_map(&m->w2, k4, 4, cache + H * I, dims, strides, box, true))) return s;
+  }
+  // weight scales of rows that are 16-byte multiples (the strides' unit)
+  const uint8_t* scales = cache + 3 * H * I / 2;
+  if (H % 512 == 0) {
+    const cuuint64_t dims[4] = {H / 32, I, 2, slots};
+    const cuuint64_t strides[3] = {H / 32, I * (H / 32), row_bytes};
+    const cuuint32_t box[4] = {16, kMxFeatures, 2, 1};
+    if ((s = make_map(&m->s1, k8, 4, scales, dims, strides, box, false))) return s;
+  }
+  if (I % 512 == 0) {
+    const cuuint64_t dims[3] = {I / 32, H, slots};
+    const cuuint64_t strides[2] = {I / 32, row_bytes};
+    const cuuint32_t box[3] = {16, kMxM, 1};
+    if ((s = make_map(&m->s2, k8, 3, scales + 2 * I * (H / 32), dims, strides, box, false))) return s;
+  }
+  for (int c = 0; c < 4; ++c) {
+    const cuuint32_t box[4] = {kStepK, 16u << c, 2, kSpan};
+    for (int phase = 0; phase < 2; ++phase) {
+      const cuuint64_t K = phase ? I : H;
+      const cuuint64_t dims[4] = {kStepK, routes, 2, K / kStepK};
+      const cuuint64_t strides[3] = {2 * K, K, kStepK};
+      if ((s = make_map(phase ? &m->a[c] : &m->x[c], k8, 4, phase ? act : x, dims, strides, box, true)))
+        return s;
+    }
+  }
+  for (int phase = 0; phase < 2; ++phase) {
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(phase ? pitch2 : pitch1), routes};
+    const cuuint64_t strides[1] = {dims[0]};
+    const cuuint32_t box[2] = {16, 16};
+    if ((s = make_map(phase ? &m->as : &m->xs, k8, 2, phase ? as : xs, dims, strides, box, false))) return s;
+  }
   return FERRYB_OK;
 }
 
@@ -1083,30 +1147,19 @@ extern "C" int ferryb_execute_experts_mxfp4(const ferryb_mxfp4_experts_args* e, 
   int device = 0;
   FB_CUDA(cudaGetDevice(&device));
   const int sms = num_sms(device);
-  MxMaps maps;
-  const int64_t hi = e->hidden * e->intermediate, row_bytes = 3 * hi / 32 * 17;
-  const uint8_t* cache = static_cast<const uint8_t*>(e->cache);
-  if ((s = make_map_codes(&maps.w1, cache, e->hidden, 2 * e->intermediate, e->cache_slots, row_bytes,
-                          kMxFeatures)))
-    return s;
-  if ((s = make_map_codes(&maps.w2, cache + hi, e->intermediate, e->hidden, e->cache_slots, row_bytes,
-                          kMxM)))
-    return s;
-  if ((s = make_map_bytes(&maps.x16, base + ws.x, e->routes, 2 * e->hidden, kStepK, 16))) return s;
-  if ((s = make_map_bytes(&maps.x64, base + ws.x, e->routes, 2 * e->hidden, kStepK, 64))) return s;
-  if ((s = make_map_bytes(&maps.a16, base + ws.act, e->routes, 2 * e->intermediate, kStepK, 16))) return s;
-  if ((s = make_map_bytes(&maps.a64, base + ws.act, e->routes, 2 * e->intermediate, kStepK, 64))) return s;
-  if ((s = make_map_bytes(&maps.xs, base + ws.xs, e->routes, ws.pitch1, 16, 16))) return s;
-  if ((s = make_map_bytes(&maps.as, base + ws.as, e->routes, ws.pitch2, 16, 16))) return s;
+  MxMaps maps{};
+  if ((s = make_maps(&maps, e, pr.x, base + ws.act, pr.xs, base + ws.as, ws.pitch1, ws.pitch2))) return s;
   MxParams p{};
   p.groups = pr.groups;
   p.header = pr.header;
   p.mt1 = static_cast<int>(e->intermediate / kMxFeatures);
   p.mt2 = static_cast<int>(e->hidden / kMxM);
+  p.tma1 = e->hidden % 512 == 0;
+  p.tma2 = e->intermediate % 512 == 0;
   p.hidden = static_cast<int>(e->hidden);
   p.inter = static_cast<int>(e->intermediate);
-  p.scales = cache + 3 * hi / 2;
-  p.row_bytes = row_bytes;
+  p.scales = static_cast<const uint8_t*>(e->cache) + 3 * e->hidden * e->intermediate / 2;
+  p.row_bytes = 3 * e->hidden * e->intermediate / 32 * 17;
   p.act = base + ws.act;
   p.as = base + ws.as;
   p.pitch2 = static_cast<int>(ws.pitch2);
