@@ -139,7 +139,8 @@ def scatter_returned(returned, send_idx, tokens):
 
 def _cuda_call(device, name, *args):
     """call() on `device`'s current stream, whatever the current device is."""
-    stream = stream_ptr(device)
+    # the raw stream costs a tenth of a microsecond, a torch.cuda.Stream three
+    stream = torch._C._cuda_getCurrentRawStream(device.index)
     if device.index == torch.cuda.current_device():
         call(name, *args, stream)
     else:
@@ -154,8 +155,11 @@ def _same_device(device, **tensors):
 
 
 def _dense_rows(t):
-    """t itself if the values of a row are adjacent, else a contiguous copy."""
-    return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+    """2-D t itself if the values of a row are adjacent and its rows do not
+    overlap, else a contiguous copy."""
+    rows, width = t.shape
+    stride, step = t.stride()
+    return t if (step == 1 or width <= 1) and (stride >= width or rows <= 1) else t.contiguous()
 
 
 SCORES = {'softmax': 0, 'sigmoid': 1}
@@ -179,11 +183,15 @@ def route_experts(logits, topk, *, score='softmax', bias=None, n_group=1, topk_g
     and give NaN weights.  Scores are compared in 64 bits.  At most 1024
     experts, topk <= 32, n_group <= 32."""
     require_cuda(logits, bias)
-    _check(logits.dim() == 2 and logits.dtype in _lib.ELEMENT_TYPES,
-           'logits must be bf16, fp16 or float32 [tokens, experts]')
-    _check(score in SCORES, f'score must be one of {sorted(SCORES)}')
-    _check(group_score in GROUP_SCORES, f'group_score must be one of {sorted(GROUP_SCORES)}')
-    _check(weights_dtype in _lib.ELEMENT_TYPES, 'weights_dtype must be bf16, fp16 or float32')
+    logits_type, weights_type = _lib.ELEMENT_TYPES.get(logits.dtype), _lib.ELEMENT_TYPES.get(weights_dtype)
+    if logits_type is None or logits.dim() != 2:
+        raise _lib.FerrybError('logits must be bf16, fp16 or float32 [tokens, experts]')
+    if weights_type is None:
+        raise _lib.FerrybError('weights_dtype must be bf16, fp16 or float32')
+    if score not in SCORES:
+        raise _lib.FerrybError(f'score must be one of {sorted(SCORES)}')
+    if group_score not in GROUP_SCORES:
+        raise _lib.FerrybError(f'group_score must be one of {sorted(GROUP_SCORES)}')
     tokens, experts = logits.shape
     dev = logits.device
     if bias is not None:
@@ -191,15 +199,13 @@ def route_experts(logits, topk, *, score='softmax', bias=None, n_group=1, topk_g
         _same_device(dev, bias=bias)
         bias = bias.contiguous()
     logits = _dense_rows(logits)
-    if tokens > 1 and logits.stride(0) < experts:
-        logits = logits.contiguous()
     topk = int(topk)
-    _check(0 < topk <= experts, f'topk must be in [1, {experts}]')
-    selected = torch.empty((tokens, topk), dtype=torch.int64, device=dev)
-    weights = torch.empty((tokens, topk), dtype=weights_dtype, device=dev)
+    if not 0 < topk <= experts:
+        raise _lib.FerrybError(f'topk must be in [1, {experts}]')
+    selected = logits.new_empty((tokens, topk), dtype=torch.int64)
+    weights = logits.new_empty((tokens, topk), dtype=weights_dtype)
     args = _lib.RouteArgs(logits.data_ptr(), tokens, logits.stride(0), experts, topk, int(n_group),
-                          int(topk_group), _lib.ELEMENT_TYPES[logits.dtype],
-                          _lib.ELEMENT_TYPES[weights_dtype], SCORES[score], GROUP_SCORES[group_score],
+                          int(topk_group), logits_type, weights_type, SCORES[score], GROUP_SCORES[group_score],
                           int(bool(norm_topk_prob)), float(scaling), _lib.addr(bias),
                           selected.data_ptr(), weights.data_ptr())
     _cuda_call(dev, 'ferryb_route_experts', ctypes.byref(args))
@@ -208,28 +214,31 @@ def route_experts(logits, topk, *, score='softmax', bias=None, n_group=1, topk_g
 
 def _rows_2d(t, name):
     """t as [rows, width] without a copy, the values of a row adjacent."""
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+    if t.dim() != 2:
+        try:
+            t = t.view(-1, t.shape[-1])
+        except RuntimeError:
+            raise _lib.FerrybError(f'{name}: the rows must be evenly spaced, their values adjacent') from None
+    rows, width = t.shape
+    stride, step = t.stride()
+    if step != 1 and width > 1:
         raise _lib.FerrybError(f'{name}: the values of a row must be adjacent')
-    try:
-        t = t.view(-1, t.shape[-1]) if t.dim() != 2 else t
-    except RuntimeError:
-        raise _lib.FerrybError(f'{name}: the rows must be evenly spaced') from None
-    if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+    if stride < width and rows > 1:
         raise _lib.FerrybError(f'{name}: rows overlap')
     return t
 
 
-def _mxfp4_out(out, shape, device):
-    """(codes, scales) for values of `shape`: `out` checked, or new tensors."""
-    lead, width = tuple(shape[:-1]), shape[-1]
+def _mxfp4_out(out, x):
+    """(codes, scales) for the values of x: `out` checked, or new tensors."""
+    *lead, width = x.shape
     if out is None:
-        return (torch.empty(lead + (width // 2,), dtype=torch.uint8, device=device),
-                torch.empty(lead + (width // 32,), dtype=torch.uint8, device=device))
+        return (x.new_empty((*lead, width // 2), dtype=torch.uint8),
+                x.new_empty((*lead, width // 32), dtype=torch.uint8))
     codes, scales = out
     for name, t, n in (('codes', codes, width // 2), ('scales', scales, width // 32)):
-        _check(t.dtype == torch.uint8 and tuple(t.shape) == lead + (n,),
-               f'{name} must be uint8 {list(lead + (n,))}, got {t.dtype} {list(t.shape)}')
-        _same_device(device, **{name: t})
+        if t.dtype != torch.uint8 or t.shape != (*lead, n):
+            raise _lib.FerrybError(f'{name} must be uint8 {[*lead, n]}, got {t.dtype} {list(t.shape)}')
+        _same_device(x.device, **{name: t})
     return codes, scales
 
 
@@ -244,18 +253,19 @@ def quantize_mxfp4(x, out=None):
     a NaN has s = 255 and reads back as NaN.  `out`: (codes, scales) to write
     to, such as the two parts of expert rows (ferry_b200.model.mxfp4_parts)."""
     require_cuda(x)
-    _check(x.dim() >= 1 and x.dtype in _lib.ELEMENT_TYPES, 'x must be bf16, fp16 or float32')
+    kind = _lib.ELEMENT_TYPES.get(x.dtype)
+    if kind is None or x.dim() < 1:
+        raise _lib.FerrybError('x must be bf16, fp16 or float32')
     width = x.shape[-1]
-    _check(width % 32 == 0, f'the last dimension ({width}) must be a multiple of 32')
-    codes, scales = _mxfp4_out(out, x.shape, x.device)
+    if width % 32:
+        raise _lib.FerrybError(f'the last dimension ({width}) must be a multiple of 32')
+    codes, scales = _mxfp4_out(out, x)
     if x.numel() == 0:
         return codes, scales
-    x2 = _dense_rows(x).reshape(-1, width)
-    if x2.shape[0] > 1 and x2.stride(0) < width:
-        x2 = x2.contiguous()
+    x2 = _dense_rows(x if x.dim() == 2 else x.reshape(-1, width))
     c2, s2 = _rows_2d(codes, 'codes'), _rows_2d(scales, 'scales')
-    _cuda_call(x.device, 'ferryb_quantize_mxfp4', ptr(x2), _lib.ELEMENT_TYPES[x.dtype], x2.shape[0], width,
-               x2.stride(0), ptr(c2), c2.stride(0), ptr(s2), s2.stride(0))
+    _cuda_call(x.device, 'ferryb_quantize_mxfp4', x2.data_ptr(), kind, x2.shape[0], width, x2.stride(0),
+               c2.data_ptr(), c2.stride(0), s2.data_ptr(), s2.stride(0))
     return codes, scales
 
 
@@ -263,25 +273,27 @@ def dequantize_mxfp4(codes, scales, dtype=BF16, out=None):
     """The values of quantize_mxfp4's codes and scales, rounded once to `dtype`
     (bf16 and float32 hold them exactly, but for 6 * 2^127 and its like)."""
     require_cuda(codes, scales, out)
-    _check(codes.dim() >= 1 and codes.dtype == torch.uint8 and scales.dtype == torch.uint8,
-           'codes and scales must be uint8')
-    lead, width = tuple(codes.shape[:-1]), 2 * codes.shape[-1]
-    _check(width % 32 == 0 and tuple(scales.shape) == lead + (width // 32,),
-           f'codes {list(codes.shape)} need scales {list(lead + (width // 32,))} (blocks of 32 values), '
-           f'got {list(scales.shape)}')
-    _check(dtype in _lib.ELEMENT_TYPES, 'dtype must be bf16, fp16 or float32')
+    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.dim() < 1:
+        raise _lib.FerrybError('codes and scales must be uint8')
+    *lead, half = codes.shape
+    width = 2 * half
+    if width % 32 or scales.shape != (*lead, width // 32):
+        raise _lib.FerrybError(f'codes {list(codes.shape)} need scales {[*lead, width // 32]} '
+                               f'(blocks of 32 values), got {list(scales.shape)}')
+    kind = _lib.ELEMENT_TYPES.get(dtype)
+    if kind is None:
+        raise _lib.FerrybError('dtype must be bf16, fp16 or float32')
     _same_device(codes.device, scales=scales, out=out)
     if out is None:
-        out = torch.empty(lead + (width,), dtype=dtype, device=codes.device)
-    _check(out.dtype == dtype and tuple(out.shape) == lead + (width,),
-           f'out must be {dtype} {list(lead + (width,))}')
+        out = codes.new_empty((*lead, width), dtype=dtype)
+    elif out.dtype != dtype or out.shape != (*lead, width):
+        raise _lib.FerrybError(f'out must be {dtype} {[*lead, width]}')
     if out.numel() == 0:
         return out
     o2 = _rows_2d(out, 'out')
-    c2, s2 = (_dense_rows(t).reshape(-1, t.shape[-1]) for t in (codes, scales))
-    c2, s2 = (t if t.shape[0] <= 1 or t.stride(0) >= t.shape[1] else t.contiguous() for t in (c2, s2))
-    _cuda_call(codes.device, 'ferryb_dequantize_mxfp4', ptr(c2), c2.stride(0), ptr(s2), s2.stride(0),
-               o2.shape[0], width, ptr(o2), _lib.ELEMENT_TYPES[dtype], o2.stride(0))
+    c2, s2 = (_dense_rows(t if t.dim() == 2 else t.reshape(-1, t.shape[-1])) for t in (codes, scales))
+    _cuda_call(codes.device, 'ferryb_dequantize_mxfp4', c2.data_ptr(), c2.stride(0), s2.data_ptr(), s2.stride(0),
+               o2.shape[0], width, o2.data_ptr(), kind, o2.stride(0))
     return out
 
 
@@ -306,52 +318,55 @@ def execute_experts_mxfp4(cache, input, routing_weights, slots, starts, rows, co
     that starts at 0, it returns at once and leaves a non-zero code there for
     the caller to check, and can be captured into a CUDA graph."""
     require_cuda(cache, input, routing_weights, slots, starts, rows, cols, out, err)
-    hidden, intermediate = int(hidden), int(intermediate)
-    _check(hidden > 0 and intermediate > 0 and hidden % 128 == 0 and intermediate % 128 == 0,
-           f'hidden ({hidden}) and intermediate ({intermediate}) must be multiples of 128')
     dev = input.device
     _same_device(dev, cache=cache, routing_weights=routing_weights, slots=slots, starts=starts, rows=rows,
                  cols=cols, out=out, err=err)
+    hidden, intermediate = int(hidden), int(intermediate)
+    if hidden <= 0 or intermediate <= 0 or hidden % 128 or intermediate % 128:
+        raise _lib.FerrybError(f'hidden ({hidden}) and intermediate ({intermediate}) must be multiples of 128')
     row_bytes = 3 * hidden * intermediate // 32 * 17
-    _check(cache.dtype == torch.uint8 and cache.dim() == 2 and cache.shape[1] == row_bytes
-           and cache.is_contiguous() and cache.data_ptr() % 32 == 0,
-           f'cache must be contiguous 32-byte aligned uint8 [slots, {row_bytes}]')
-    _check(input.dtype == BF16 and input.dim() == 2 and input.shape[1] == hidden,
-           f'input must be bf16 [n, {hidden}]')
-    _check(routing_weights.dim() == 2 and routing_weights.shape[0] == input.shape[0]
-           and routing_weights.dtype in _lib.ELEMENT_TYPES,
-           'routing_weights must be bf16, fp16 or float32 [n, topk]')
+    if (cache.dtype != torch.uint8 or cache.dim() != 2 or cache.shape[1] != row_bytes
+            or not cache.is_contiguous() or cache.data_ptr() % 32):
+        raise _lib.FerrybError(f'cache must be contiguous 32-byte aligned uint8 [slots, {row_bytes}]')
+    if input.dtype != BF16 or input.dim() != 2 or input.shape[1] != hidden:
+        raise _lib.FerrybError(f'input must be bf16 [n, {hidden}]')
+    tokens = input.shape[0]
+    weights_type = _lib.ELEMENT_TYPES.get(routing_weights.dtype)
+    if weights_type is None or routing_weights.dim() != 2 or routing_weights.shape[0] != tokens:
+        raise _lib.FerrybError('routing_weights must be bf16, fp16 or float32 [n, topk]')
     for name, t in (('slots', slots), ('starts', starts), ('rows', rows), ('cols', cols)):
-        _check(t.dtype == torch.int64 and t.dim() == 1, f'{name} must be a 1-D int64 tensor')
+        if t.dtype != torch.int64 or t.dim() != 1:
+            raise _lib.FerrybError(f'{name} must be a 1-D int64 tensor')
     groups, routes = slots.shape[0], rows.shape[0]
-    _check(starts.shape[0] == groups + 1, f'starts must have {groups + 1} entries (one more than slots)')
+    if starts.shape[0] != groups + 1:
+        raise _lib.FerrybError(f'starts must have {groups + 1} entries (one more than slots)')
     _check(cols.shape[0] == routes, 'rows and cols must have equal length')
     if out is None:
-        out = torch.empty((routes, hidden), dtype=BF16, device=dev)
-    _check(out.dtype == BF16 and tuple(out.shape) == (routes, hidden) and out.is_contiguous(),
-           f'out must be contiguous bf16 [{routes}, {hidden}]')
+        out = input.new_empty((routes, hidden))
+    elif out.dtype != BF16 or out.shape != (routes, hidden) or not out.is_contiguous():
+        raise _lib.FerrybError(f'out must be contiguous bf16 [{routes}, {hidden}]')
     wait = err is None
     if not wait:
         _check(err.dtype == torch.int32 and err.numel() == 1, 'err must be an int32 tensor of one element')
     if routes == 0 or groups == 0:
         return out
     _check(cache.shape[0] > 0, 'cache has no slots')
-    if input.stride(1) != 1 or input.data_ptr() % 16 or (input.shape[0] > 1 and (
-            input.stride(0) % 8 or input.stride(0) < hidden)):
+    stride, step = input.stride()
+    if step != 1 or input.data_ptr() % 16 or tokens > 1 and (stride % 8 or stride < hidden):
         input = input.clone(memory_format=torch.contiguous_format)
+        stride = hidden
     routing_weights = routing_weights.contiguous()
-    slots, starts, rows, cols = (t.contiguous() for t in (slots, starts, rows, cols))
+    slots, starts, rows, cols = slots.contiguous(), starts.contiguous(), rows.contiguous(), cols.contiguous()
     ws_bytes = _lib.lib().ferryb_execute_experts_mxfp4_workspace(routes, groups, hidden, intermediate)
     if ws_bytes < 0:
         raise _lib.FerrybError(_lib.lib().ferryb_last_error().decode())
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    ws = cache.new_empty((ws_bytes,))
     if wait:
         err = torch.zeros(1, dtype=torch.int32, device=dev)
     args = _lib.Mxfp4ExpertsArgs(
-        cache.data_ptr(), cache.shape[0], input.data_ptr(), input.shape[0], input.stride(0),
-        routing_weights.data_ptr(), routing_weights.shape[1], _lib.ELEMENT_TYPES[routing_weights.dtype], 0,
-        slots.data_ptr(), starts.data_ptr(), groups, rows.data_ptr(), cols.data_ptr(), routes, hidden,
-        intermediate, out.data_ptr(), ws.data_ptr(), ws_bytes, err.data_ptr())
+        cache.data_ptr(), cache.shape[0], input.data_ptr(), tokens, stride, routing_weights.data_ptr(),
+        routing_weights.shape[1], weights_type, 0, slots.data_ptr(), starts.data_ptr(), groups, rows.data_ptr(),
+        cols.data_ptr(), routes, hidden, intermediate, out.data_ptr(), ws.data_ptr(), ws_bytes, err.data_ptr())
     _cuda_call(dev, 'ferryb_execute_experts_mxfp4', ctypes.byref(args))
     if wait:
         _lib.check_device_error(err, 'execute_experts_mxfp4')
