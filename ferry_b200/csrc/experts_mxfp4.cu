@@ -21,9 +21,9 @@
 // within 2^-9 of its value (bf16: 2^-9), or 2^-21 of its block's largest.  Gate, up and silu stay in float32, the result is rounded
 // to bf16 once.
 //
-// Orientation as in experts.cu: 128 weight rows are the MMA's M side (64 gate
-// rows above the 64 up rows of the same features, or 128 down rows), the routes
-// its N side.  Groups are split into sub-groups of at most 32, 64 or 128 routes
+// Orientation as in experts.cu: 128 weight rows are the MMA's M side (four times
+// 16 gate rows and the 16 up rows of the same features, so that a feature's gate
+// and up meet in one warp; or 128 down rows), the routes its N side.  Groups are split into sub-groups of at most 32, 64 or 128 routes
 // (by the mean of the groups: small groups need no wide tiles, and narrow ones
 // leave shared memory to the weights), each with its own work items, so that a
 // popular expert is spread over the GPU.
@@ -37,11 +37,14 @@
 // each 32 columns of the step); one thread issues the 8 MMAs of K = 32, hi and
 // lo for each scale byte.
 //
-// CTA roles (512 threads): warp 0 claims work and loads codes; warp 1 issues the
-// MMAs; warps 2-5 and 6-9 drain the two accumulators; warp 10 loads the routes;
-// warp 15 brings the weights' scales, warps 11-14 move all scales on.  Codes do not depend on phase
-// 1, so warp 0 runs ahead into phase 2 while the routes' warps wait for the
-// activations.
+// CTA roles (352 threads): warp 0 claims work and loads codes; warp 1 issues the
+// MMAs; warps 2-5 drain the accumulators; warp 6 loads the routes; warps 9 and
+// 10 bring the weights' and the routes' scales, warps 7 and 8 arrange them.
+// Codes do not depend on phase 1, so warps 0 and 9 run ahead into phase 2 while
+// the routes' warps wait for the activations.  Two CTAs share an SM: what bounds
+// a CTA is the one thread behind each load or MMA (measured: a wait that is
+// already over 100 cycles, an expect 40, a TMA load 290, an MMA or scale copy
+// 45, a commit 85), and two have two of each.
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
@@ -52,27 +55,34 @@
 
 namespace ferryb {
 
-constexpr int kMxWarps = 16;
-constexpr int kMxThreads = kMxWarps * 32;
-constexpr int kFirstEpi = 2, kRouteWarp = 10, kFirstScale = 11, kScaleLoad = 15;
 constexpr int kMxM = 128;          // weight rows per tile
-constexpr int kMxN = 128;          // most routes of a sub-group
 constexpr int kStepK = 128;        // columns per step
-constexpr int kSpan = 2;           // steps per load and barrier
 constexpr int kMxFeatures = 64;    // gate (= up) rows per phase-1 tile
-constexpr int kBars = 8;           // barriers of the spans' pipeline, more than any buffer's depth
+constexpr int kBars = 8;           // barriers of the step pipeline, more than any buffer's depth
 constexpr int kBlock = 4;          // steps whose scales come in one piece and are arranged by one warp
-constexpr int kPieces = 4;         // places for a block's scales as they are in memory
-constexpr uint32_t kStepCodes = kMxM * kStepK;  // a step's codes, unpacked
-constexpr uint32_t kCodeBytes = kSpan * kStepCodes;
-constexpr uint32_t kPieceBytes = kMxM * 16;  // of up to four steps
-constexpr uint32_t kScalePool = 24 * 1024;  // scales as they are in memory, and arranged
-constexpr uint32_t kTmemScale = 256;  // first TMEM column of the scales: four places of 16 columns
+constexpr int kPlaces = 2;         // such pieces in shared memory, one for each of two warps
+constexpr uint32_t kTileCodes = kMxM * kStepK;  // a step's codes of one tile, unpacked
+constexpr uint32_t kPieceBytes = kMxM * 16;     // scale bytes of four steps of 128 rows
 constexpr int kRing = 4;           // claimed items in flight
-constexpr int kXStride = 9;        // floats a feature of the gate/up exchange (padded)
-constexpr uint32_t kXchgBytes = 2 * kMxFeatures * kXStride * 4;  // an epilogue group's
-constexpr uint32_t kPoolBytes = 12 * 16384;  // codes and routes
-constexpr uint32_t kMxSmem = kPoolBytes + kScalePool + 1024 + 1024;
+constexpr uint32_t kXchgBytes = 2 * 4 * 16;  // exponents of 16 columns from four warps, twice
+constexpr uint32_t kBarBytes = 512;
+
+constexpr int kTiles = 2;          // tiles of weight rows per item
+// warps: 0 claims and codes, 1 and 2 MMAs of a tile each, then
+constexpr int kFirstEpi = 3, kEpiWarps = 4 * kTiles, kRouteWarp = kFirstEpi + kEpiWarps, kFirstScale = kRouteWarp + 1,
+              kScaleLoad = kFirstScale + 2, kRouteScale = kScaleLoad + 1;
+constexpr int kMxThreads = (kRouteScale + 1) * 32;
+constexpr int kItemReaders = 2 + kEpiWarps + 5;
+constexpr uint32_t kCodeBytes = kTiles * kTileCodes;
+constexpr uint32_t kPoolBytes = 196 * 1024;        // codes and routes
+constexpr uint32_t kTilePool = 12 * 1024;          // arranged scales
+// tensor memory: two accumulators of two tiles of 112 columns, then the scales: two
+// places of two times 12 columns (weights', hi, lo) where hi and lo are apart,
+// else four of two times 8
+constexpr uint32_t kTmemCols = 512, kTileCols = 112, kAccCols = kTiles * kTileCols, kTmemScale = 2 * kAccCols;
+constexpr uint32_t kMxSmem =
+    kPoolBytes + kPlaces * (kTiles + 1) * kPieceBytes + kTilePool + kTiles * kXchgBytes + kBarBytes;
+static_assert(kMxSmem <= 227 * 1024, "shared memory");
 constexpr uint64_t kMxWaitNs = 2000000000ull;  // bound on any wait
 
 // Up to 128 routes of one group.
@@ -87,13 +97,14 @@ struct MxGroup {
 struct MxHeader {
   int queue;     // claim counter
   int n_groups;  // sub-groups
-  int box;       // 0..3: sub-groups of at most 16, 32, 64, 128 routes
+  int cap;       // most routes of a sub-group: 16, 48 or 112
 };
 
 struct MxParams {
   const MxGroup* groups;
   MxHeader* header;
-  int mt1, mt2;         // items per sub-group: I / 64 phase 1, H / 128 phase 2
+  int mt1, mt2;         // items per sub-group, each of two tiles: I / 64 tiles phase 1, H / 128 phase 2
+  int t1, t2;           // those tiles
   int tma1, tma2;       // weight scales of phase 1 (2) through s1 (s2): rows of 16-byte multiples
   int hidden, inter;
   const uint8_t* scales;  // slot 0's scale bytes
@@ -109,7 +120,7 @@ struct MxParams {
 
 struct MxMaps {
   CUtensorMap w1, w2;      // codes of gate and up rows, of down rows
-  CUtensorMap x[4], a[4];  // routes and activations, 16, 32, 64, 128 rows at once
+  CUtensorMap x[7], a[7];  // routes and activations: 16, 32, ... 112 rows at once
   CUtensorMap xs, as;      // their scale bytes [routes, pitch], 16 rows x 16 bytes at once
   CUtensorMap s1, s2;      // scale bytes of gate and up rows, of down rows, 16 bytes of 128 rows
 };
@@ -188,14 +199,6 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, u
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
       : "memory");
 }
-__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int32_t c0,
-                                            int32_t c1, int32_t c2, int32_t c3) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
-      : "memory");
-}
 __device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, uint64_t* bar, int32_t c0,
                                             int32_t c1, int32_t c2, int32_t c3, int32_t c4) {
   asm volatile(
@@ -227,30 +230,46 @@ __device__ __forceinline__ uint64_t smem_desc_scales(uint32_t saddr) {
 __device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint64_t desc) {
   asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
-// 32 lanes x 8 consecutive columns of 32 bits.
-__device__ __forceinline__ void tmem_ld8(uint32_t taddr, float* v) {
-  uint32_t r[8];
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-                 "=r"(r[7])
-               : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
+// 32 lanes x 16 consecutive columns of 32 bits; tmem_ld_wait before they are used.
+__device__ __forceinline__ void tmem_ld16_start(uint32_t taddr, float* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32"
+      " {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]),
+        "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]),
+        "=f"(v[14]), "=f"(v[15])
+      : "r"(taddr));
+}
+// The values pass through, so that no use of them moves before the wait.
+__device__ __forceinline__ void tmem_ld_wait(float* v) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]),
+                 "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]),
+                 "+f"(v[14]), "+f"(v[15])
+               :
+               : "memory");
 }
 
 // D[tmem] (+)= (A[smem] * scales) x (B[smem] * scales)^T, 32 columns: e2m1 codes
 // in 8-bit places times e4m3, float32 accumulate, one UE8M0 scale for the 32.
+// KEEP 1 leaves A in the tensor core's buffer, for the next MMA with the same A,
+// KEEP 2, which does not read it from shared memory again.
+template <int KEEP>
 __device__ __forceinline__ void umma_mxf8f6f4(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc,
                                               uint32_t idesc, uint32_t sfa, uint32_t sfb,
                                               uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %6, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], "
-      "p;\n\t}" ::"r"(tmem_d),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-      : "memory");
+#define FB_UMMA(collector)                                                                              \
+  asm volatile(                                                                                         \
+      "{\n\t.reg .pred p;\n\t"                                                                          \
+      "setp.ne.b32 p, %6, 0;\n\t"                                                                       \
+      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X" collector                     \
+      " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(tmem_d),                                           \
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)                           \
+      : "memory")
+  if (KEEP == 0) FB_UMMA("");
+  else if (KEEP == 1) FB_UMMA(".collector::a::fill");
+  else FB_UMMA(".collector::a::lastuse");
+#undef FB_UMMA
 }
 // Instruction descriptor of kind::mxf8f6f4: A e2m1 (5 in bits 7-9), B e4m3 (0 in
 // bits 10-12), both K-major, N >> 3 in bits 17-22, UE8M0 scales (bit 23), M >> 7
@@ -260,21 +279,21 @@ __device__ __forceinline__ uint32_t mx_idesc(uint32_t n, uint32_t byte) {
   return (5u << 7) | ((n >> 3) << 17) | (1u << 23) | (1u << 27) | (byte << 4) | (byte << 29);
 }
 
-// A step: its scales into tensor memory, then four K = 32 MMAs (eight with WIDE:
-// hi, then lo into the same columns).  Descriptors count in 16 bytes: 32 columns
-// are 2, 512 bytes of scales 32, the 128 rows of a wide hi part 1024.
-template <bool WIDE>
-__device__ __forceinline__ void issue_step(uint32_t d, uint64_t a, uint64_t b, uint32_t b_off, uint32_t sa,
-                                           uint64_t from, uint32_t idesc, bool accumulate) {
-  tmem_copy_scales(sa, from);
-  tmem_copy_scales(sa + 4, from + 32);
-  if (WIDE) tmem_copy_scales(sa + 8, from + 64);
-  b += b_off;
+// A tile's step: its scales into tensor memory, then four K = 32 MMAs (eight where
+// hi and lo go into the same columns, one after the other).  Descriptors count in
+// 16 bytes: 32 columns are 2, 512 bytes of scales 32; `lo` is the distance of the
+// lo part, `bs` the routes' scales.
+template <bool SPLIT>
+__device__ __forceinline__ void issue_step(uint32_t d, uint64_t a, uint64_t b, uint64_t lo, uint32_t sa,
+                                           uint64_t as, uint64_t bs, uint32_t idesc, bool accumulate) {
+  tmem_copy_scales(sa, as);
+  tmem_copy_scales(sa + 4, bs);
+  if (SPLIT) tmem_copy_scales(sa + 8, bs + 32);
 #pragma unroll
   for (uint32_t k = 0; k < 4; ++k) {
     const uint32_t id = idesc | (k << 4) | (k << 29);
-    umma_mxf8f6f4(d, a + 2 * k, b + 2 * k, id, sa, sa + 4, accumulate || k > 0 ? 1u : 0u);
-    if (WIDE) umma_mxf8f6f4(d, a + 2 * k, b + 1024 + 2 * k, id, sa, sa + 8, 1u);
+    umma_mxf8f6f4<SPLIT ? 1 : 0>(d, a + 2 * k, b + 2 * k, id, sa, sa + 4, accumulate || k > 0 ? 1u : 0u);
+    if (SPLIT) umma_mxf8f6f4<2>(d, a + 2 * k, b + lo + 2 * k, id, sa, sa + 8, 1u);
   }
 }
 
@@ -298,13 +317,10 @@ __device__ __forceinline__ void mx_split2(float a, float b, uint32_t* hi, uint32
   *lo = l;
 }
 
-// The four warps of epilogue group g (0 or 1) meet at named barrier 1 + g, and
-// leave their loop together: every decision goes through a barrier that ANDs
-// it.
-__device__ __forceinline__ void mx_epilogue_sync(int g) {
-  asm volatile("bar.sync %0, 128;" ::"r"(1 + g) : "memory");
-}
-__device__ __forceinline__ bool mx_epilogue_all(int g, bool v) {
+// A tile's four epilogue warps meet at their named barrier, and leave their loop
+// together: every decision goes through a barrier that ANDs it.
+__device__ __forceinline__ void mx_epilogue_sync(int id) { asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ bool mx_epilogue_all(int id, bool v) {
   uint32_t r;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
@@ -312,39 +328,29 @@ __device__ __forceinline__ bool mx_epilogue_all(int g, bool v) {
       "bar.red.and.pred q, %2, 128, p;\n\t"
       "selp.u32 %0, 1, 0, q;\n\t}"
       : "=r"(r)
-      : "r"(static_cast<uint32_t>(v)), "r"(1 + g)
+      : "r"(static_cast<uint32_t>(v)), "r"(id)
       : "memory");
   return r != 0;
 }
 
 // The pool of shared memory, by the sub-groups' size: places of codes first, then
-// places of routes (hi and lo parts of `box` rows), a span each.  Many places
+// places of routes (hi and lo parts of `cap` rows), a step each.  More places
 // for codes where routes are few (memory-bound), as many of both where they
 // are many.
-__host__ __device__ __forceinline__ int mx_code_stages(int box) {
-  return box == 0 ? 5 : box == 1 ? 4 : box == 2 ? 3 : 2;
-}
-__host__ __device__ __forceinline__ int mx_route_stages(int box) {
-  return box == 0 ? 4 : box == 1 ? 4 : box == 2 ? 3 : 2;
-}
-__host__ __device__ __forceinline__ uint32_t mx_route_bytes(int box) {
-  return (16u << box) * kStepK * 2 * kSpan;
-}
+__device__ __forceinline__ uint32_t mx_code_stages(int cap) { return cap <= 48 ? 5 : 3; }
+__device__ __forceinline__ uint32_t mx_route_stages(int cap) { return cap == 16 ? 4 : 3; }
 
-// Rows of routes that a sub-group's tile holds: 16, 32, 64 or 128.
-__device__ __forceinline__ int mx_class(int count) {
-  return count <= 16 ? 0 : count <= 32 ? 1 : count <= 64 ? 2 : 3;
-}
-__device__ __forceinline__ int mx_rows(int count) { return 16 << mx_class(count); }
+// Rows of routes that a sub-group's tile holds: the next multiple of 16.
+__device__ __forceinline__ int mx_rows(int count) { return (count + 15) & ~15; }
+// Hi and lo side by side in one MMA of twice the columns (added up in the
+// epilogue), so that the weights are read once, as far as the accumulators have
+// room; else one after the other into the same columns.
+__device__ __forceinline__ bool mx_split(int rows) { return rows > 48; }
 
-// A span is two steps: loads, barriers and commits cost the one thread that
-// issues them 100 to 300 cycles each (a TMA load alone 290, the next one behind
-// it 50), which by the step was more than the step's 375 cycles of HBM time.
-// Spans are numbered from 0 over all items of a CTA (an item's last span may be
-// half empty: zeros).  Span t uses barrier t % 8 of each pipeline; a buffer of S
-// places may be refilled for span t once span t - S is done, and S < 8 keeps the
-// parity unambiguous.
-__device__ __forceinline__ bool mx_wait_span(uint64_t* bars, uint32_t t, volatile int* abort_flag,
+// Steps are numbered from 0 over all items of a CTA.  Step t uses barrier t % 8
+// of each pipeline; a buffer of S places may be refilled for step t once step t
+// - S is done, and S < 8 keeps the parity unambiguous.
+__device__ __forceinline__ bool mx_wait_step(uint64_t* bars, uint32_t t, volatile int* abort_flag,
                                              int* err) {
   return mx_wait(bars + t % kBars, (t / kBars) & 1, abort_flag, err);
 }
@@ -370,58 +376,63 @@ __device__ __forceinline__ bool mx_wait_dep(const int* dep, uint32_t want, volat
 
 __global__ void __launch_bounds__(kMxThreads, 1)
     mxfp4_swiglu_kernel(const __grid_constant__ MxMaps maps, const MxParams p) {
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
-                                             ~uintptr_t(1023));
-  uint8_t* scale = smem + kPoolBytes;  // places of weights' scales [128 rows] 16 bytes
-  uint64_t* full = reinterpret_cast<uint64_t*>(scale + kScalePool);
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if (smem_u32(smem) % 1024 != 0) {  // the swizzled tiles rely on it
+    if (threadIdx.x == 0) atomicCAS(p.err, 0, DEV_LAYOUT_OVERFLOW);
+    return;
+  }
+  uint8_t* scale = smem + kPoolBytes;  // [kPlaces] weights' scales, 16 bytes of 128 * kTiles rows
+  uint8_t* rscale = scale + kPlaces * kTiles * kPieceBytes;  // [kPlaces] the same of the routes
+  uint8_t* tiles = rscale + kPlaces * kPieceBytes;  // a step's arranged scales each
+  uint8_t* xchg = tiles + kTilePool;
+  uint64_t* full = reinterpret_cast<uint64_t*>(xchg + kTiles * kXchgBytes);
   uint64_t* done = full + kBars;     // the MMAs of a step are complete
-  uint64_t* kfull = done + kBars;    // [kPieces] a block's scales landed
-  uint64_t* kempty = kfull + kPieces;
-  uint64_t* tfull = kempty + kPieces;  // [2] accumulators
-  uint64_t* tempty = tfull + 2;
-  uint64_t* ifull = tempty + 2;      // [kRing] claimed items
+  uint64_t* kfull = done + kBars;    // [kPlaces] a block's scales landed
+  uint64_t* kempty = kfull + kPlaces;
+  uint64_t* tfull = kempty + kPlaces;  // [tile][2] accumulators
+  uint64_t* tempty = tfull + 2 * kTiles;
+  uint64_t* ifull = tempty + 2 * kTiles;      // [kRing] claimed items
   uint64_t* iempty = ifull + kRing;
   uint64_t* drain = iempty + kRing;
   uint32_t* tmem_smem = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_smem + 1);
   MxItem* ring = reinterpret_cast<MxItem*>(drain + 2);  // [kRing]
-  __shared__ float xchg_all[2][kXchgBytes / 4];
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (threadIdx.x == 0) {
     for (int s = 0; s < kBars; ++s) {
       mbar_init(&full[s], 3);  // codes, routes and scales
-      mbar_init(&done[s], 1);
+      mbar_init(&done[s], kTiles);
     }
-    for (int s = 0; s < kPieces; ++s) {
-      mbar_init(&kfull[s], 33);  // TMA, and the lanes' cp.async
+    for (int s = 0; s < kPlaces; ++s) {
+      mbar_init(&kfull[s], 34);  // both loaders' TMA, and the lanes' cp.async
       mbar_init(&kempty[s], 1);
     }
-    for (int b = 0; b < 2; ++b) { mbar_init(&tfull[b], 1); mbar_init(&tempty[b], 4); }
-    for (int q = 0; q < kRing; ++q) { mbar_init(&ifull[q], 1); mbar_init(&iempty[q], 11 + (p.header->box == 3 ? 2 : 4)); }
-    mbar_init(drain, 1);
+    for (int b = 0; b < 2 * kTiles; ++b) { mbar_init(&tfull[b], 1); mbar_init(&tempty[b], 4); }
+    for (int q = 0; q < kRing; ++q) { mbar_init(&ifull[q], 1); mbar_init(&iempty[q], kItemReaders); }
+    mbar_init(drain, kTiles);
     *abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == 1) { tmem_alloc(tmem_smem, 512); tmem_relinquish(); }
+  if (warp == 1) { tmem_alloc(tmem_smem, kTmemCols); tmem_relinquish(); }
+  if (warp == 0 && lane < 4) {
+    tma_prefetch_desc(lane == 0 ? &maps.w1 : lane == 1 ? &maps.w2 : lane == 2 ? &maps.xs : &maps.as);
+    tma_prefetch_desc(&maps.x[lane]);
+    tma_prefetch_desc(&maps.a[lane]);
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_smem;
-  const int box = p.header->box;
-  const uint32_t code_stages = mx_code_stages(box), route_stages = mx_route_stages(box);
-  const uint32_t route_bytes = mx_route_bytes(box);
+  pdl_wait();  // what follows reads the prepare kernel's tables
+  const int cap = p.header->cap;
+  const uint32_t code_stages = mx_code_stages(cap), route_stages = mx_route_stages(cap);
+  const uint32_t route_bytes = cap * kStepK * 2;
   uint8_t* const routes = smem + code_stages * kCodeBytes;
-  // Blocks go around the scale warps, each of which has a place of its own for
-  // the weights' and for the routes' bytes.  Arranged, a step has 512 bytes of
-  // weights' scales, 512 of routes' and, for 128 routes, 512 of lo scales: more,
-  // and two warps (and places) instead of four.
-  const uint32_t places = box == 3 ? 2 : 4, tile_bytes = box == 3 ? 1536 : 1024;
-  const uint32_t place_bytes = box == 3 ? kPieceBytes : kPieceBytes / 2;  // of the routes
-  uint8_t* const rscale = scale + places * kPieceBytes;
-  uint8_t* const tiles = rscale + places * place_bytes;
-  const uint32_t tile_spans = box == 3 ? 5 : 6;
+  // arranged, a step has 512 bytes of scales for each tile, 512 for the routes and,
+  // where hi and lo are apart, 512 of lo scales
+  const uint32_t tile_bytes = (kTiles + 1 + mx_split(cap)) * 512;
+  const uint32_t n_tiles = min(kTilePool / tile_bytes, 6u);
   int q = 0;            // this role's place in the item ring
   uint32_t qphase = 0;
 
@@ -430,7 +441,7 @@ __global__ void __launch_bounds__(kMxThreads, 1)
     if (elect_one()) {
       uint32_t t = 0, stage = 0;
       bool ok = true;
-      const int n_groups = p.header->n_groups;
+      const int first = atomicAdd(&p.header->queue, 1), n_groups = p.header->n_groups;
       auto publish = [&](const MxItem& it) {
         if (!mx_wait(&iempty[q], qphase ^ 1, abort_flag, p.err)) return false;
         ring[q] = it;
@@ -438,7 +449,7 @@ __global__ void __launch_bounds__(kMxThreads, 1)
         if (++q == kRing) { q = 0; qphase ^= 1; }
         return true;
       };
-      MxItem it = mx_item(p, n_groups, atomicAdd(&p.header->queue, 1));
+      MxItem it = mx_item(p, n_groups, first);
       ok = publish(it);
       while (ok && it.phase != 0) {
         // the next item is claimed now and published a few loads on, before this
@@ -446,18 +457,17 @@ __global__ void __launch_bounds__(kMxThreads, 1)
         const int id = atomicAdd(&p.header->queue, 1);
         MxItem next{};
         const int K = it.phase == 1 ? p.hidden : p.inter;
-        const int row0 = it.tile * (it.phase == 1 ? kMxFeatures : kMxM);
-        const int steps = K / kStepK, ahead = steps > kSpan ? kSpan : 0;
-        for (int kb = 0; kb < steps; kb += kSpan, ++t) {
-          if (t >= code_stages && !mx_wait_span(done, t - code_stages, abort_flag, p.err)) {
+        const int steps = K / kStepK, ahead = min(steps - 1, 3);
+        for (int kb = 0; kb < steps; ++kb, ++t) {
+          if (t >= code_stages && !mx_wait_step(done, t - code_stages, abort_flag, p.err)) {
             ok = false;
             break;
           }
           uint64_t* bar = full + t % kBars;
           uint8_t* cs = smem + stage * kCodeBytes;
           mbar_expect_tx(bar, kCodeBytes / 2);  // the copy counts its 4-bit data, not the gaps
-          if (it.phase == 1) tma_load_5d(cs, &maps.w1, bar, 0, row0, 0, kb, it.slot);
-          else tma_load_4d(cs, &maps.w2, bar, 0, row0, kb, it.slot);
+          if (it.phase == 1) tma_load_5d(cs, &maps.w1, bar, kb * kStepK, 0, 0, it.tile * 4 * kTiles, it.slot);
+          else tma_load_3d(cs, &maps.w2, bar, kb * kStepK, it.tile * kMxM * kTiles, it.slot);
           if (++stage == code_stages) stage = 0;
           if (kb == ahead) {
             next = mx_item(p, n_groups, id);
@@ -475,15 +485,12 @@ __global__ void __launch_bounds__(kMxThreads, 1)
       }
     }
   } else if (warp == kScaleLoad) {
-    // ---------------- scales into shared memory ----------------
-    // Its own warp: the scales of a block go through more hands than the codes
-    // and routes of its steps, and start their way earlier.
+    // ---------------- weights' scales into shared memory ----------------
     uint32_t place = 0, ph = 0;
     bool ok = true;
     while (ok) {
       if (!mx_wait_warp(&ifull[q], qphase, abort_flag, p.err)) break;
-      const int phase = ring[q].phase, tile = ring[q].tile, slot = ring[q].slot, group = ring[q].group;
-      const int start = ring[q].start, rows = mx_rows(ring[q].count);
+      const int phase = ring[q].phase, tile = ring[q].tile, slot = ring[q].slot;
       __syncwarp();
       if (lane == 0) mbar_arrive(&iempty[q]);
       if (++q == kRing) { q = 0; qphase ^= 1; }
@@ -491,55 +498,71 @@ __global__ void __launch_bounds__(kMxThreads, 1)
       const int K = phase == 1 ? p.hidden : p.inter;
       // 16 bytes (four steps) of each tile row: one TMA load where the rows are
       // 16-byte multiples (K a multiple of 512), else cp.async of 8 or 4 bytes, rows
-      // lane + 32 * i
+      // lane + 32 * i (16 gate rows, 16 up rows, ...)
       const bool tma = (phase == 1 ? p.tma1 : p.tma2) != 0;
       const int pitch = K / 32;
+      const int row = phase == 1 ? (lane < 16 ? 0 : p.inter) + tile * kMxFeatures * kTiles + (lane & 15)
+                                 : tile * kMxM * kTiles + lane;
+      const int parts = min(4 * kTiles, 4 * ((phase == 1 ? p.t1 : p.t2) - tile * kTiles));  // of 32 rows
       const uint8_t* src = p.scales + slot * p.row_bytes +
                            (phase == 1 ? 0 : 2 * static_cast<int64_t>(p.inter) * (p.hidden / 32)) +
-                           static_cast<int64_t>(tile * (phase == 1 ? kMxFeatures : kMxM) + lane) * pitch;
-      const int64_t d1 = 32 * pitch;
-      const int64_t d2 = phase == 1 ? static_cast<int64_t>(p.inter) * pitch : 2 * d1;  // up rows
-      if (phase == 2) {
-        bool there = true;
-        if (lane == 0) there = mx_wait_dep(p.dep + group, 4 * p.mt1, abort_flag, p.err);
-        if (!__shfl_sync(0xffffffffu, there, 0)) break;
-        asm volatile("fence.proxy.async.global;" ::: "memory");
-      }
+                           static_cast<int64_t>(row) * pitch;
+      const int64_t d1 = (phase == 1 ? 16 : 32) * pitch;
       for (int b = 0; b < pitch; b += 16) {
         if (!mx_wait_warp(&kempty[place], ph ^ 1, abort_flag, p.err)) { ok = false; break; }
-        uint8_t* to = scale + place * kPieceBytes;
+        uint8_t* to = scale + place * kTiles * kPieceBytes;
         if (lane == 0) {
-          mbar_expect_tx(&kfull[place], rows * 16 + (tma ? kPieceBytes : 0));
-          if (tma && phase == 1) tma_load_4d(to, &maps.s1, &kfull[place], b, tile * kMxFeatures, 0, slot);
-          else if (tma) tma_load_3d(to, &maps.s2, &kfull[place], b, tile * kMxM, slot);
-          for (int i = 0; i < rows; i += 16)
-            tma_load_2d(rscale + place * place_bytes + i * 16, phase == 1 ? &maps.xs : &maps.as, &kfull[place], b,
-                        start + i);
+          mbar_expect_tx(&kfull[place], tma ? kTiles * kPieceBytes : 0);
+          if (tma && phase == 1) tma_load_5d(to, &maps.s1, &kfull[place], b, 0, 0, tile * 4 * kTiles, slot);
+          else if (tma) tma_load_3d(to, &maps.s2, &kfull[place], b, tile * kMxM * kTiles, slot);
         }
         __syncwarp();
         to += lane * 16;
         const uint8_t* from = src + b;
-        if (tma) {
-        } else if (pitch % 8 == 0) {
-          for (int i = 0; i < min(16, pitch - b); i += 8) {
-            cp_async<8>(to + i, from + i);
-            cp_async<8>(to + 512 + i, from + d1 + i);
-            cp_async<8>(to + 1024 + i, from + d2 + i);
-            cp_async<8>(to + 1536 + i, from + d2 + d1 + i);
-          }
-        } else {
-          for (int i = 0; i < min(16, pitch - b); i += 4) {
-            cp_async<4>(to + i, from + i);
-            cp_async<4>(to + 512 + i, from + d1 + i);
-            cp_async<4>(to + 1024 + i, from + d2 + i);
-            cp_async<4>(to + 1536 + i, from + d2 + d1 + i);
+        if (!tma) {
+          const int n = min(16, pitch - b);
+          for (int c = 0; c < parts; ++c, to += 512, from += d1) {
+            if (pitch % 8 == 0) {
+              for (int i = 0; i < n; i += 8) cp_async<8>(to + i, from + i);
+            } else {
+              for (int i = 0; i < n; i += 4) cp_async<4>(to + i, from + i);
+            }
           }
         }
         cp_async_arrive(&kfull[place]);
-        if (++place == places) { place = 0; ph ^= 1; }
+        if (++place == kPlaces) { place = 0; ph ^= 1; }
       }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
+  } else if (warp == kRouteScale) {
+    // ---------------- routes' scales into shared memory ----------------
+    // Apart from the routes: a block's scales go through more hands than the
+    // codes and routes of its steps, and start their way earlier.
+    if (elect_one()) {
+      uint32_t place = 0, ph = 0;
+      bool ok = true;
+      while (ok) {
+        if (!mx_wait(&ifull[q], qphase, abort_flag, p.err)) break;
+        const int phase = ring[q].phase, group = ring[q].group, start = ring[q].start;
+        const int rows = mx_rows(ring[q].count);
+        mbar_arrive(&iempty[q]);
+        if (++q == kRing) { q = 0; qphase ^= 1; }
+        if (phase == 0) break;
+        if (phase == 2) {
+          if (!mx_wait_dep(p.dep + group, 4 * p.t1, abort_flag, p.err)) break;
+          asm volatile("fence.proxy.async.global;" ::: "memory");
+        }
+        const int pitch = (phase == 1 ? p.hidden : p.inter) / 32;
+        const CUtensorMap* map = phase == 1 ? &maps.xs : &maps.as;
+        for (int b = 0; b < pitch; b += 16) {
+          if (!mx_wait(&kempty[place], ph ^ 1, abort_flag, p.err)) { ok = false; break; }
+          mbar_expect_tx(&kfull[place], rows * 16);
+          for (int i = 0; i < rows; i += 16)
+            tma_load_2d(rscale + place * kPieceBytes + i * 16, map, &kfull[place], b, start + i);
+          if (++place == kPlaces) { place = 0; ph ^= 1; }
+        }
+      }
+    }
   } else if (warp == kRouteWarp) {
     // ---------------- routes ----------------
     if (elect_one()) {
@@ -552,21 +575,21 @@ __global__ void __launch_bounds__(kMxThreads, 1)
         if (++q == kRing) { q = 0; qphase ^= 1; }
         if (it.phase == 0) break;
         if (it.phase == 2) {
-          if (!mx_wait_dep(p.dep + it.group, 4 * p.mt1, abort_flag, p.err)) { ok = false; break; }
+          if (!mx_wait_dep(p.dep + it.group, 4 * p.t1, abort_flag, p.err)) { ok = false; break; }
           asm volatile("fence.proxy.async.global;" ::: "memory");
         }
         const int steps = (it.phase == 1 ? p.hidden : p.inter) / kStepK;
-        const int cls = mx_class(it.count);
+        const int rows = mx_rows(it.count), cls = rows / 16 - 1;
         const CUtensorMap* map = it.phase == 1 ? &maps.x[cls] : &maps.a[cls];
-        for (int kb = 0; kb < steps; kb += kSpan, ++t) {
-          if (t >= route_stages && !mx_wait_span(done, t - route_stages, abort_flag, p.err)) {
+        for (int kb = 0; kb < steps; ++kb, ++t) {
+          if (t >= route_stages && !mx_wait_step(done, t - route_stages, abort_flag, p.err)) {
             ok = false;
             break;
           }
           uint64_t* bar = full + t % kBars;
-          mbar_expect_tx(bar, (16u << cls) * kStepK * 2 * kSpan);
-          // per step the rows' hi parts, then their lo parts
-          tma_load_4d(routes + stage * route_bytes, map, bar, 0, it.start, 0, kb);
+          mbar_expect_tx(bar, rows * kStepK * 2);
+          // the rows' hi parts, then their lo parts
+          tma_load_3d(routes + stage * route_bytes, map, bar, kb * kStepK, it.start, 0);
           if (++stage == route_stages) stage = 0;
         }
       }
@@ -581,80 +604,90 @@ __global__ void __launch_bounds__(kMxThreads, 1)
     // Into the MMA's order: row r's four bytes of a step at (r % 32) * 16 + r / 32
     // * 4.
     const uint32_t me = warp - kFirstScale;
-    uint32_t t = 0, turn = 0, ph = 0;  // spans and blocks of all items
-    bool ok = me < places;
+    uint32_t t = 0, turn = 0, tile = 0, ph = 0;  // steps and blocks of all items
+    bool ok = true;
     while (ok) {
       if (!mx_wait_warp(&ifull[q], qphase, abort_flag, p.err)) break;
       const int phase = ring[q].phase, rows = mx_rows(ring[q].count);
+      const bool split = mx_split(rows);
       __syncwarp();
       if (lane == 0) mbar_arrive(&iempty[q]);
       if (++q == kRing) { q = 0; qphase ^= 1; }
       if (phase == 0) break;
       const int steps = (phase == 1 ? p.hidden : p.inter) / kStepK;
-      for (int k = 0; k < steps; k += kBlock) {
+      for (int k = 0; k < steps && ok; k += kBlock, turn ^= 1) {
         const int n = min(kBlock, steps - k);
-        const uint32_t spans = (n + kSpan - 1) / kSpan;
-        const bool mine = turn == me;
-        if (++turn == places) turn = 0;
-        if (!mine) { t += spans; continue; }
+        if (turn != me) {
+          t += n;
+          tile = tile + n >= n_tiles ? tile + n - n_tiles : tile + n;
+          continue;
+        }
         if (!mx_wait_warp(&kfull[me], ph, abort_flag, p.err)) { ok = false; break; }
         ph ^= 1;
         // four steps of weight rows lane + 32 * c, and of routes
-        const uint4* rs = reinterpret_cast<const uint4*>(rscale + me * place_bytes);
-        const uint4* ws = reinterpret_cast<const uint4*>(scale + me * kPieceBytes);
-        uint4 b4[4], a4[4];
+        const uint4* rs = reinterpret_cast<const uint4*>(rscale + me * kPieceBytes);
+        const uint4* ws = reinterpret_cast<const uint4*>(scale + me * kTiles * kPieceBytes);
+        uint4 b4[4], a4[kTiles][4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          a4[c] = ws[lane + 32 * c];
+#pragma unroll
+          for (int i = 0; i < kTiles; ++i) a4[i][c] = ws[i * 128 + lane + 32 * c];
+          // columns of the MMA: the rows' hi parts and, side by side, their lo parts
+          const int r = lane + 32 * c;
           b4[c] = make_uint4(0, 0, 0, 0);
-          if (c == 0) b4[c] = rs[rows == 16 ? lane & 15 : lane];
-          else if (rows > 32 * c) b4[c] = rs[lane + 32 * c];
+          if (r < rows) b4[c] = rs[r];
+          else if (!split && r < 2 * rows) b4[c] = rs[r - rows];
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&kempty[me]);
-        // the tiles' last users are done
-        if (t + spans > tile_spans &&
-            !__all_sync(0xffffffffu, mx_wait_span(done, t + spans - 1 - tile_spans, abort_flag, p.err))) {
-          ok = false;
-          break;
-        }
 #pragma unroll
         for (int i = 0; i < kBlock; ++i) {
-          if (i < n) {
+          if (i < n && ok) {
             auto part = [&](const uint4& v) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; };
             // the lo scales are 2^-4 of the hi ones (every byte is at least 4)
             constexpr uint32_t kLo = 0x04040404u;
             uint4 b = make_uint4(part(b4[0]), part(b4[1]), part(b4[2]), part(b4[3]));
-            uint4* to = reinterpret_cast<uint4*>(
-                            tiles + (((t + i / kSpan) % tile_spans) * kSpan + i % kSpan) * tile_bytes) + lane;
-            if (rows == 16) {
-              if (lane >= 16) b.x -= kLo;
-            } else if (rows == 32) {
-              b.y = b.x - kLo;
-            } else if (rows == 64) {
-              b.z = b.x - kLo;
-              b.w = b.y - kLo;
-            } else {
-              to[64] = make_uint4(b.x - kLo, b.y - kLo, b.z - kLo, b.w - kLo);
+            const uint4 low = make_uint4(b.x - kLo, b.y - kLo, b.z - kLo, b.w - kLo);
+            if (!split) {
+              if (lane >= rows) b.x = low.x;
+              if (lane + 32 >= rows) b.y = low.y;
+              if (lane + 64 >= rows) b.z = low.z;
+              if (lane + 96 >= rows) b.w = low.w;
             }
-            to[0] = make_uint4(part(a4[0]), part(a4[1]), part(a4[2]), part(a4[3]));
-            to[32] = b;
+            // the tile's last user is done
+            if (t >= n_tiles &&
+                !__all_sync(0xffffffffu, mx_wait_step(done, t - n_tiles, abort_flag, p.err))) {
+              ok = false;
+            } else {
+              uint4* to = reinterpret_cast<uint4*>(tiles + tile * tile_bytes) + lane;
+#pragma unroll
+              for (int u = 0; u < kTiles; ++u)
+                to[32 * u] = make_uint4(part(a4[u][0]), part(a4[u][1]), part(a4[u][2]), part(a4[u][3]));
+              to[32 * kTiles] = b;
+              if (split) to[32 * kTiles + 32] = low;
+              fence_proxy_async();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&full[t % kBars]);
+              ++t;
+              if (++tile == n_tiles) tile = 0;
+            }
           }
         }
-        fence_proxy_async();
-        __syncwarp();
-        if (lane < static_cast<int>(spans)) mbar_arrive(&full[(t + lane) % kBars]);
-        t += spans;
       }
     }
-  } else if (warp == 1) {
+  } else if (warp < kFirstEpi) {
     // ---------------- MMA ----------------
+    // One warp for each tile: the thread that waits, issues and commits would
+    // bound a step that had both.
     if (elect_one()) {
-      uint32_t t = 0, cstage = 0, rstage = 0, tspan = 0;
-      const uint64_t a0 = smem_desc_sw128(smem_u32(smem)), b0 = smem_desc_sw128(smem_u32(routes));
+      const uint32_t part = warp - 1;
+      uint32_t t = 0, cstage = 0, rstage = 0, tile = 0;
+      const uint64_t a0 = smem_desc_sw128(smem_u32(smem + part * kTileCodes)), b0 = smem_desc_sw128(smem_u32(routes));
       const uint64_t s0 = smem_desc_scales(smem_u32(tiles));
-      int acc = 0;
-      uint32_t acc_phase = 0;
+      const bool apart = mx_split(cap);
+      uint32_t acc = 0, acc_phase = 0;
+      tfull += 2 * part;
+      tempty += 2 * part;
       bool ok = true;
       while (ok) {
         if (!mx_wait(&ifull[q], qphase, abort_flag, p.err)) break;
@@ -663,35 +696,24 @@ __global__ void __launch_bounds__(kMxThreads, 1)
         mbar_arrive(&iempty[q]);
         if (++q == kRing) { q = 0; qphase ^= 1; }
         if (kind == 0) break;
-        // up to 64 routes: hi and lo side by side in one MMA of twice the columns
-        // (added up in the epilogue), so that the weights are read once; 128: one
-        // after the other into the same columns
-        const bool wide = rows == 128;
-        const uint32_t idesc = mx_idesc(wide ? 128 : 2 * rows, 0);
+        const bool split = mx_split(rows);
+        const uint32_t idesc = mx_idesc(split ? rows : 2 * rows, 0);
         const int steps = (kind == 1 ? p.hidden : p.inter) / kStepK;
         if (!mx_wait(&tempty[acc], acc_phase ^ 1, abort_flag, p.err)) break;
         tc_fence_after();
-        const uint32_t d = tmem + acc * kMxN;
-        for (int kb = 0; kb < steps; kb += kSpan, ++t) {
-          if (!mx_wait_span(full, t, abort_flag, p.err)) { ok = false; break; }
+        const uint32_t d = tmem + acc * kAccCols + part * kTileCols;
+        for (int kb = 0; kb < steps; ++kb, ++t) {
+          if (!mx_wait_step(full, t, abort_flag, p.err)) { ok = false; break; }
           tc_fence_after();
           const uint64_t a = a0 + cstage * (kCodeBytes >> 4), b = b0 + rstage * (route_bytes >> 4);
-          const uint32_t sa = tmem + kTmemScale + (t & 1) * (kSpan * 16);
-          const uint64_t from = s0 + tspan * (kSpan * tile_bytes >> 4);
-          if (wide) {
-            issue_step<true>(d, a, b, 0, sa, from, idesc, kb > 0);
-            if (kb + 1 < steps)
-              issue_step<true>(d, a + (kStepCodes >> 4), b, 256 * kStepK >> 4, sa + 16, from + (1536 >> 4), idesc, true);
-          } else {
-            issue_step<false>(d, a, b, 0, sa, from, idesc, kb > 0);
-            if (kb + 1 < steps)
-              issue_step<false>(d, a + (kStepCodes >> 4), b, rows * (2 * kStepK >> 4), sa + 16, from + (tile_bytes >> 4),
-                                idesc, true);
-          }
+          const uint32_t sa = tmem + kTmemScale + (apart ? (t & 1) * 24 + part * 12 : (t & 3) * 16 + part * 8);
+          const uint64_t from = s0 + tile * (tile_bytes >> 4);
+          if (split) issue_step<true>(d, a, b, rows * 8, sa, from + part * 32, from + kTiles * 32, idesc, kb > 0);
+          else issue_step<false>(d, a, b, 0, sa, from + part * 32, from + kTiles * 32, idesc, kb > 0);
           umma_commit(&done[t % kBars]);
           if (++cstage == code_stages) cstage = 0;
           if (++rstage == route_stages) rstage = 0;
-          if (++tspan == tile_spans) tspan = 0;
+          if (++tile == n_tiles) tile = 0;
         }
         if (!ok) break;
         umma_commit(&tfull[acc]);
@@ -703,105 +725,108 @@ __global__ void __launch_bounds__(kMxThreads, 1)
       while (!mbar_try_wait(drain, 0) && globaltimer_ns() - t0 < kMxWaitNs) {}
     }
   } else {
-    // ---------------- epilogue (warps 2..9) ----------------
-    // group 0 drains accumulator 0, group 1 accumulator 1: every other item.
-    // TMEM lanes 32 * (warp % 4)..: quarters 0, 1 hold gate rows of a phase-1
-    // tile, 2, 3 the up rows of the same features
-    const int eg = (warp - kFirstEpi) >> 2;
-    const int qd = warp & 3;
-    const bool up_rows = qd >= 2;
-    const int f_local = (qd & 1) * 32 + lane;
-    float* xchg = xchg_all[eg];
-    float* give = xchg + (up_rows ? kMxFeatures * kXStride : 0) + f_local * kXStride;
-    const float* take = xchg + (up_rows ? 0 : kMxFeatures * kXStride) + f_local * kXStride;
-    uint32_t acc_phase = 0;
-    for (int turn = 0;; turn ^= 1) {
-      if (!mx_epilogue_all(eg, mx_wait(&ifull[q], qphase, abort_flag, p.err))) break;
+    // ---------------- epilogue (four warps for each tile) ----------------
+    // TMEM lanes 32 * (warp % 4)..: 16 gate rows of a phase-1 tile and the 16 up
+    // rows of the same features, or 32 down rows
+    const int qd = warp & 3, part = (warp - kFirstEpi) / 4, bar = 1 + part;
+    tfull += 2 * part;
+    tempty += 2 * part;
+    xchg += part * kXchgBytes;
+    const bool low = lane < 16;
+    uint32_t turn = 0;
+    uint32_t acc = 0, acc_phase = 0;
+    for (;;) {
+      if (!mx_epilogue_all(bar, mx_wait(&ifull[q], qphase, abort_flag, p.err))) break;
       const MxItem it = ring[q];
       __syncwarp();
       if (lane == 0) mbar_arrive(&iempty[q]);
       if (++q == kRing) { q = 0; qphase ^= 1; }
       if (it.phase == 0) break;  // the same entry for all four warps
-      if (turn != eg) continue;
+      const int tile = it.tile * kTiles + part;
+      const bool mine = tile < (it.phase == 1 ? p.t1 : p.t2);  // the last item may lack a tile
       // routing weights of routes lane, lane + 32, ... (phase 2)
       float w[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c)
         w[c] = it.bad ? __uint_as_float(0x7fc00000u)
                : it.phase == 2 && lane + 32 * c < it.count ? p.route_w[it.start + lane + 32 * c] : 0.0f;
-      if (!mx_epilogue_all(eg, mx_wait(&tfull[eg], acc_phase, abort_flag, p.err))) break;
-      acc_phase ^= 1;
+      if (!mx_epilogue_all(bar, mx_wait(&tfull[acc], acc_phase, abort_flag, p.err))) break;
       tc_fence_after();
-      const uint32_t d = tmem + (static_cast<uint32_t>(qd * 32) << 16) + eg * kMxN;
-      // 8 columns from c0 on: the hi part's sums, plus the lo part's where they
+      const uint32_t d = tmem + (static_cast<uint32_t>(qd * 32) << 16) + acc * kAccCols + part * kTileCols;
+      // 16 columns from c0 on: the hi part's sums, plus the lo part's where they
       // have columns of their own
-      const int lo_at = it.count > 64 ? 0 : mx_rows(it.count);
+      const int lo_at = mx_split(mx_rows(it.count)) ? 0 : mx_rows(it.count);
       auto columns = [&](int c0, float* v) {
-        tmem_ld8(d + c0, v);
+        tmem_ld16_start(d + c0, v);
         if (lo_at) {
-          float more[8];
-          tmem_ld8(d + lo_at + c0, more);
+          float more[16];
+          tmem_ld16_start(d + lo_at + c0, more);
+          tmem_ld_wait(more);
+          tmem_ld_wait(v);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] += more[j];
+          for (int j = 0; j < 16; ++j) v[j] += more[j];
+        } else {
+          tmem_ld_wait(v);
         }
       };
-      if (it.phase == 1) {
-        // 16 routes at a time: gate warps finish the first 8, up warps the rest
-        const int block = it.tile * 2 + (qd & 1);  // of 32 features
-        for (int c0 = 0; c0 < it.count; c0 += 16) {
-          float lo[8], hi[8];
-          columns(c0, lo);
-          columns(c0 + 8, hi);
+      if (!mine) {
+      } else if (it.phase == 1) {
+        // 16 routes at a time, in pairs: a feature's gate lane takes the even one, its
+        // up lane the odd one, each handing the other the value it needs.  The scale
+        // of 32 features is two warps': they exchange exponents, by turns in two
+        // places, so that one barrier does.
+        for (int c0 = 0; c0 < it.count; c0 += 16, turn ^= 1) {
+          float v[16], a[8];
+          uint32_t top[8], h[4], l[4];
+          columns(c0, v);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) give[j] = up_rows ? lo[j] : hi[j];
-          mx_epilogue_sync(eg);
-          const int first = c0 + (up_rows ? 8 : 0);
-          const int n = it.count - first;  // of these 8 routes
-          if (n > 0) {
-            // no branches between the routes: 8 independent chains
-            float a[8];
-            uint32_t top[8], h[4], l[4];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const float gate = up_rows ? take[j] : lo[j];
-              const float up = up_rows ? hi[j] : take[j];
-              a[j] = __fdividef(gate, 1.0f + __expf(-gate)) * up;
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              top[j] = __reduce_max_sync(0xffffffffu, __float_as_uint(a[j]) & 0x7fffffffu);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              top[j] = mx_block_byte(top[j] >> 23);
-              a[j] *= mx_block_mult(top[j]);
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) mx_split2(a[2 * j], a[2 * j + 1], &h[j], &l[j]);
-            uint8_t* to = p.act + static_cast<int64_t>(it.start + first) * (2 * p.inter) +
-                          it.tile * kMxFeatures + f_local;
-            uint8_t* sb = p.as + static_cast<int64_t>(it.start + first) * p.pitch2 + block;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              if (j < n) {
-                to[0] = static_cast<uint8_t>(j & 1 ? h[j / 2] >> 8 : h[j / 2]);
-                to[p.inter] = static_cast<uint8_t>(j & 1 ? l[j / 2] >> 8 : l[j / 2]);
-                if (lane == 0) sb[0] = static_cast<uint8_t>(top[j]);
-              }
-              to += 2 * p.inter;
-              sb += p.pitch2;
-            }
+          for (int j = 0; j < 8; ++j) {
+            const float other = __shfl_xor_sync(0xffffffffu, low ? v[2 * j + 1] : v[2 * j], 16);
+            const float gate = low ? v[2 * j] : other, up = low ? other : v[2 * j + 1];
+            a[j] = __fdividef(gate, 1.0f + __expf(-gate)) * up;
           }
-          mx_epilogue_sync(eg);
+          uint8_t* ex = xchg + turn * 64;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const uint32_t e = (__float_as_uint(a[j]) >> 23) & 255u;
+            const uint32_t even = __reduce_max_sync(0xffffffffu, low ? e : 0u);
+            const uint32_t odd = __reduce_max_sync(0xffffffffu, low ? 0u : e);
+            top[j] = low ? even : odd;
+            if ((lane & 15) == 0) ex[qd * 16 + 2 * j + (lane >> 4)] = static_cast<uint8_t>(top[j]);
+          }
+          mx_epilogue_sync(bar);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            top[j] = max(top[j], static_cast<uint32_t>(ex[(qd ^ 1) * 16 + 2 * j + (lane >> 4)]));
+            top[j] = mx_block_byte(top[j]);
+            a[j] *= mx_block_mult(top[j]);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) mx_split2(a[2 * j], a[2 * j + 1], &h[j], &l[j]);
+          const int first = c0 + (lane >> 4);
+          uint8_t* to = p.act + static_cast<int64_t>(it.start + first) * (2 * p.inter) +
+                        tile * kMxFeatures + qd * 16 + (lane & 15);
+          uint8_t* sb = p.as + static_cast<int64_t>(it.start + first) * p.pitch2 + tile * 2 + (qd >> 1);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            if (first + 2 * j < it.count) {
+              to[0] = static_cast<uint8_t>(j & 1 ? h[j / 2] >> 8 : h[j / 2]);
+              to[p.inter] = static_cast<uint8_t>(j & 1 ? l[j / 2] >> 8 : l[j / 2]);
+              if ((lane & 15) == 0 && (qd & 1) == 0) sb[0] = static_cast<uint8_t>(top[j]);
+            }
+            to += 4 * p.inter;
+            sb += 2 * p.pitch2;
+          }
         }
       } else {
-        __nv_bfloat16* to = p.out + static_cast<int64_t>(it.start) * p.hidden + it.tile * kMxM + qd * 32 + lane;
-        for (int c0 = 0; c0 < it.count; c0 += 8) {
-          float v[8];
+        __nv_bfloat16* to = p.out + static_cast<int64_t>(it.start) * p.hidden + tile * kMxM + qd * 32 + lane;
+        for (int c0 = 0; c0 < it.count; c0 += 16) {
+          float v[16];
           columns(c0, v);
           const float ws = c0 < 32 ? w[0] : c0 < 64 ? w[1] : c0 < 96 ? w[2] : w[3];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float wj = __shfl_sync(0xffffffffu, ws, (c0 & 24) + j);
+          for (int j = 0; j < 16; ++j) {
+            const float wj = __shfl_sync(0xffffffffu, ws, (c0 & 16) + j);
             if (c0 + j < it.count) *to = __float2bfloat16_rn(v[j] * wj);
             to += p.hidden;
           }
@@ -809,8 +834,9 @@ __global__ void __launch_bounds__(kMxThreads, 1)
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&tempty[eg]);
-      if (it.phase == 1) {
+      if (lane == 0) mbar_arrive(&tempty[acc]);
+      if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+      if (it.phase == 1 && mine) {
         // publish this warp's activations to the sub-group's phase-2 items
         __threadfence();
         __syncwarp();
@@ -823,7 +849,7 @@ __global__ void __launch_bounds__(kMxThreads, 1)
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(tmem, kTmemCols);
   }
 }
 
@@ -857,6 +883,7 @@ constexpr int kPrepThreads = 256;
 
 __global__ void __launch_bounds__(kPrepThreads) mxfp4_prepare_kernel(const MxPrepare a) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  pdl_launch_dependents();  // the GEMM's CTAs may set up and wait
   if (blockIdx.x == 0) {
     __shared__ int warp_sum[kPrepThreads / 32];
     __shared__ int base;
@@ -872,7 +899,7 @@ __global__ void __launch_bounds__(kPrepThreads) mxfp4_prepare_kernel(const MxPre
     if (threadIdx.x == 0) { base = 0; a.header->queue = 0; }
     ordered = __syncthreads_and(ordered);
     if (!ordered) {
-      if (threadIdx.x == 0) { a.header->n_groups = 0; a.header->box = 0; atomicCAS(a.err, 0, DEV_BAD_INPUT); }
+      if (threadIdx.x == 0) { a.header->n_groups = 0; a.header->cap = 16; atomicCAS(a.err, 0, DEV_BAD_INPUT); }
       return;
     }
     atomicAdd(&base, active);
@@ -880,10 +907,10 @@ __global__ void __launch_bounds__(kPrepThreads) mxfp4_prepare_kernel(const MxPre
     active = base;
     __syncthreads();
     if (threadIdx.x == 0) base = 0;
-    // sub-groups no wider than the mean group asks for, in one of four sizes
+    // sub-groups no wider than the mean group asks for
     const int64_t all = a.starts[a.n_groups] - a.starts[0];
     const int64_t mean = active ? (all + active - 1) / active : 0;
-    const int cap = mean <= 4 ? 16 : mean <= 24 ? 32 : mean <= 48 ? 64 : 128;
+    const int cap = mean <= 4 ? 16 : mean <= 16 ? 48 : 112;
     __syncthreads();
     for (int g0 = 0; g0 < a.n_groups; g0 += kPrepThreads) {
       const int g = g0 + threadIdx.x;
@@ -921,7 +948,7 @@ __global__ void __launch_bounds__(kPrepThreads) mxfp4_prepare_kernel(const MxPre
     }
     if (threadIdx.x == 0) {
       a.header->n_groups = base;
-      a.header->box = cap == 16 ? 0 : cap == 32 ? 1 : cap == 64 ? 2 : 3;
+      a.header->cap = cap;
     }
     return;
   }
@@ -949,29 +976,37 @@ __global__ void __launch_bounds__(kPrepThreads) mxfp4_prepare_kernel(const MxPre
     uint2* to = reinterpret_cast<uint2*>(a.x + i * 2 * a.hidden);
     uint8_t* sb = a.xs + i * a.pitch1;
     // 8 values a lane, a block of 32 in four neighbours (hidden is a multiple of
-    // 128: whole blocks, and the lanes of a block are all in or all out)
-    for (int v0 = 0; v0 < a.hidden / 8; v0 += 32) {
-      const int v = v0 + lane;
-      const bool in = v < a.hidden / 8;
-      uint4 e = make_uint4(0, 0, 0, 0);
-      if (in && good) e = from[v];
-      const uint32_t m = __vmaxu2(__vmaxu2(e.x & 0x7fff7fffu, e.y & 0x7fff7fffu),
-                                  __vmaxu2(e.z & 0x7fff7fffu, e.w & 0x7fff7fffu));
-      uint32_t top = max(m & 0xffffu, m >> 16);
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const int byte = mx_block_byte(top >> 7);
-      const float mult = mx_block_mult(byte);
-      const uint32_t in8[4] = {e.x, e.y, e.z, e.w};
-      uint32_t h[4], l[4];
+    // 128: whole blocks, and the lanes of a block are all in or all out); four
+    // loads in flight
+    const int n8 = a.hidden / 8;
+    for (int v0 = 0; v0 < n8; v0 += 4 * 32) {
+      uint4 e4[4];
 #pragma unroll
-      for (int i2 = 0; i2 < 4; ++i2)
-        mx_split2(__uint_as_float(in8[i2] << 16) * mult, __uint_as_float(in8[i2] & 0xffff0000u) * mult,
-                  &h[i2], &l[i2]);
-      if (in) {
-        to[v] = make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
-        to[a.hidden / 8 + v] = make_uint2(l[0] | (l[1] << 16), l[2] | (l[3] << 16));
-        if ((v & 3) == 0) sb[v >> 2] = static_cast<uint8_t>(byte);
+      for (int u = 0; u < 4; ++u) {
+        e4[u] = make_uint4(0, 0, 0, 0);
+        if (good && v0 + u * 32 + lane < n8) e4[u] = from[v0 + u * 32 + lane];
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int v = v0 + u * 32 + lane;
+        const uint32_t in8[4] = {e4[u].x, e4[u].y, e4[u].z, e4[u].w};
+        const uint32_t m = __vmaxu2(__vmaxu2(in8[0] & 0x7fff7fffu, in8[1] & 0x7fff7fffu),
+                                    __vmaxu2(in8[2] & 0x7fff7fffu, in8[3] & 0x7fff7fffu));
+        uint32_t top = max(m & 0xffffu, m >> 16);
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int byte = mx_block_byte(top >> 7);
+        const float mult = mx_block_mult(byte);
+        uint32_t h[4], l[4];
+#pragma unroll
+        for (int i2 = 0; i2 < 4; ++i2)
+          mx_split2(__uint_as_float(in8[i2] << 16) * mult, __uint_as_float(in8[i2] & 0xffff0000u) * mult,
+                    &h[i2], &l[i2]);
+        if (v < n8) {
+          to[v] = make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+          to[n8 + v] = make_uint2(l[0] | (l[1] << 16), l[2] | (l[3] << 16));
+          if ((v & 3) == 0) sb[v >> 2] = static_cast<uint8_t>(byte);
+        }
       }
     }
   }
@@ -993,10 +1028,9 @@ static int make_map(CUtensorMap* map, CUtensorMapDataType type, int rank, const 
 }
 
 // All maps of a call.  Codes are 4-bit elements, unpacked on the way (16 codes
-// to 16 bytes of shared memory, 8 of them data).  A column index is split into
-// steps of 128 and the column inside, so that one load brings a span: for
-// each of its steps the tile's rows (gate rows, then up rows; for routes the hi
-// parts, then the lo parts), 128 columns each.
+// to 16 bytes of shared memory, 8 of them data).  One load brings a step's tile:
+// four times 16 gate rows and their 16 up rows, or 128 down rows; for routes the
+// hi parts, then the lo parts.
 static int make_maps(MxMaps* m, const ferryb_mxfp4_experts_args* e, const uint8_t* x, const uint8_t* act,
                      const uint8_t* xs, const uint8_t* as, int64_t pitch1, int64_t pitch2) {
   const cuuint64_t H = e->hidden, I = e->intermediate, slots = e->cache_slots, routes = e->routes;
@@ -1006,38 +1040,38 @@ static int make_maps(MxMaps* m, const ferryb_mxfp4_experts_args* e, const uint8_
   constexpr auto k8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
   int s;
   {
-    const cuuint64_t dims[5] = {kStepK, I, 2, H / kStepK, slots};
-    const cuuint64_t strides[4] = {H / 2, I * H / 2, kStepK / 2, row_bytes};
-    const cuuint32_t box[5] = {kStepK, kMxFeatures, 2, kSpan, 1};
+    const cuuint64_t dims[5] = {H, 16, 2, I / 16, slots};
+    const cuuint64_t strides[4] = {H / 2, I * H / 2, 16 * H / 2, row_bytes};
+    const cuuint32_t box[5] = {kStepK, 16, 2, kTiles * kMxFeatures / 16, 1};
     if ((s = make_map(&m->w1, k4, 5, cache, dims, strides, box, true))) return s;
   }
   {
-    const cuuint64_t dims[4] = {kStepK, H, I / kStepK, slots};
-    const cuuint64_t strides[3] = {I / 2, kStepK / 2, row_bytes};
-    const cuuint32_t box[4] = {kStepK, kMxM, kSpan, 1};
-    if ((s = make_map(&m->w2, k4, 4, cache + H * I, dims, strides, box, true))) return s;
+    const cuuint64_t dims[3] = {I, H, slots};
+    const cuuint64_t strides[2] = {I / 2, row_bytes};
+    const cuuint32_t box[3] = {kStepK, kTiles * kMxM, 1};
+    if ((s = make_map(&m->w2, k4, 3, cache + H * I, dims, strides, box, true))) return s;
   }
   // weight scales of rows that are 16-byte multiples (the strides' unit)
   const uint8_t* scales = cache + 3 * H * I / 2;
   if (H % 512 == 0) {
-    const cuuint64_t dims[4] = {H / 32, I, 2, slots};
-    const cuuint64_t strides[3] = {H / 32, I * (H / 32), row_bytes};
-    const cuuint32_t box[4] = {16, kMxFeatures, 2, 1};
-    if ((s = make_map(&m->s1, k8, 4, scales, dims, strides, box, false))) return s;
+    const cuuint64_t dims[5] = {H / 32, 16, 2, I / 16, slots};
+    const cuuint64_t strides[4] = {H / 32, I * (H / 32), 16 * (H / 32), row_bytes};
+    const cuuint32_t box[5] = {16, 16, 2, kTiles * kMxFeatures / 16, 1};
+    if ((s = make_map(&m->s1, k8, 5, scales, dims, strides, box, false))) return s;
   }
   if (I % 512 == 0) {
     const cuuint64_t dims[3] = {I / 32, H, slots};
     const cuuint64_t strides[2] = {I / 32, row_bytes};
-    const cuuint32_t box[3] = {16, kMxM, 1};
+    const cuuint32_t box[3] = {16, kTiles * kMxM, 1};
     if ((s = make_map(&m->s2, k8, 3, scales + 2 * I * (H / 32), dims, strides, box, false))) return s;
   }
-  for (int c = 0; c < 4; ++c) {
-    const cuuint32_t box[4] = {kStepK, 16u << c, 2, kSpan};
+  for (unsigned c = 0; c < 7; ++c) {
+    const cuuint32_t box[3] = {kStepK, 16 * (c + 1), 2};
     for (int phase = 0; phase < 2; ++phase) {
       const cuuint64_t K = phase ? I : H;
-      const cuuint64_t dims[4] = {kStepK, routes, 2, K / kStepK};
-      const cuuint64_t strides[3] = {2 * K, K, kStepK};
-      if ((s = make_map(phase ? &m->a[c] : &m->x[c], k8, 4, phase ? act : x, dims, strides, box, true)))
+      const cuuint64_t dims[3] = {K, routes, 2};
+      const cuuint64_t strides[2] = {2 * K, K};
+      if ((s = make_map(phase ? &m->a[c] : &m->x[c], k8, 3, phase ? act : x, dims, strides, box, true)))
         return s;
     }
   }
@@ -1088,6 +1122,31 @@ static int mx_sizes(int64_t routes, int64_t n_groups, int64_t hidden, int64_t in
   // the work counter is 32 bits
   FB_CHECK_ARG((n_groups + routes / 16 + 1) * (inter / 64 + hidden / 128) < (int64_t(1) << 30),
                "execute_experts_mxfp4: too many work items");
+  return FERRYB_OK;
+}
+
+static int launch_experts(const MxMaps& maps, const MxParams& p, const ferryb_mxfp4_experts_args* e, int device,
+                          cudaStream_t stream) {
+  static std::atomic<bool> attr_set[64];
+  if (device >= 64 || !attr_set[device].load(std::memory_order_acquire)) {
+    FB_CUDA(cudaFuncSetAttribute(mxfp4_swiglu_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 (int)kMxSmem));
+    if (device < 64) attr_set[device].store(true, std::memory_order_release);
+  }
+  const int64_t subs = e->n_groups < e->routes ? e->n_groups + e->routes / 16 : e->routes;
+  const int64_t items = subs * (p.mt1 + p.mt2), most = num_sms(device);
+  // programmatic dependent launch: the CTAs set up while the routes are prepared
+  cudaLaunchConfig_t lc{};
+  lc.gridDim = dim3(static_cast<unsigned>(items < most ? items : most));
+  lc.blockDim = dim3(kMxThreads);
+  lc.dynamicSmemBytes = kMxSmem;
+  lc.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  lc.attrs = &attr;
+  lc.numAttrs = 1;
+  FB_CUDA(cudaLaunchKernelEx(&lc, mxfp4_swiglu_kernel, maps, p));
   return FERRYB_OK;
 }
 
@@ -1152,8 +1211,10 @@ extern "C" int ferryb_execute_experts_mxfp4(const ferryb_mxfp4_experts_args* e, 
   MxParams p{};
   p.groups = pr.groups;
   p.header = pr.header;
-  p.mt1 = static_cast<int>(e->intermediate / kMxFeatures);
-  p.mt2 = static_cast<int>(e->hidden / kMxM);
+  p.t1 = static_cast<int>(e->intermediate / kMxFeatures);
+  p.t2 = static_cast<int>(e->hidden / kMxM);
+  p.mt1 = (p.t1 + kTiles - 1) / kTiles;
+  p.mt2 = (p.t2 + kTiles - 1) / kTiles;
   p.tma1 = e->hidden % 512 == 0;
   p.tma2 = e->intermediate % 512 == 0;
   p.hidden = static_cast<int>(e->hidden);
@@ -1172,15 +1233,5 @@ extern "C" int ferryb_execute_experts_mxfp4(const ferryb_mxfp4_experts_args* e, 
   const int64_t most = 8 * static_cast<int64_t>(sms);
   mxfp4_prepare_kernel<<<1 + static_cast<int>(gather < most ? gather : most), kPrepThreads, 0, stream>>>(pr);
   FB_LAUNCH_CHECK();
-  static std::atomic<bool> attr_set[64];
-  if (device >= 64 || !attr_set[device].load(std::memory_order_acquire)) {
-    FB_CUDA(cudaFuncSetAttribute(mxfp4_swiglu_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 (int)kMxSmem));
-    if (device < 64) attr_set[device].store(true, std::memory_order_release);
-  }
-  const int64_t subs = e->n_groups < e->routes ? e->n_groups + e->routes / 16 : e->routes;
-  const int64_t items = subs * (p.mt1 + p.mt2);
-  mxfp4_swiglu_kernel<<<static_cast<int>(items < sms ? items : sms), kMxThreads, kMxSmem, stream>>>(maps, p);
-  FB_LAUNCH_CHECK();
-  return FERRYB_OK;
+  return launch_experts(maps, p, e, device, stream);
 }
