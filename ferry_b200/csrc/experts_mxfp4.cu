@@ -64,7 +64,7 @@ constexpr int kPlaces = 2;         // such pieces in shared memory, one for each
 constexpr uint32_t kTileCodes = kMxM * kStepK;  // a step's codes of one tile, unpacked
 constexpr uint32_t kPieceBytes = kMxM * 16;     // scale bytes of four steps of 128 rows
 constexpr int kRing = 4;           // claimed items in flight
-constexpr uint32_t kXchgBytes = 2 * 4 * 16;  // exponents of 16 columns from four warps, twice
+constexpr uint32_t kXchgBytes = 2 * 4 * 32;  // magnitudes of 16 routes from four warps, twice
 constexpr uint32_t kBarBytes = 512;
 
 constexpr int kTiles = 2;          // tiles of weight rows per item
@@ -744,12 +744,13 @@ __global__ void __launch_bounds__(kMxThreads, 1)
       if (it.phase == 0) break;  // the same entry for all four warps
       const int tile = it.tile * kTiles + part;
       const bool mine = tile < (it.phase == 1 ? p.t1 : p.t2);  // the last item may lack a tile
-      // routing weights of routes lane, lane + 32, ... (phase 2)
+      // routing weights of routes lane, lane + 32, ..., with which the activations
+      // are multiplied before they are rounded
       float w[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c)
         w[c] = it.bad ? __uint_as_float(0x7fc00000u)
-               : it.phase == 2 && lane + 32 * c < it.count ? p.route_w[it.start + lane + 32 * c] : 0.0f;
+               : it.phase == 1 && lane + 32 * c < it.count ? p.route_w[it.start + lane + 32 * c] : 0.0f;
       if (!mx_epilogue_all(bar, mx_wait(&tfull[acc], acc_phase, abort_flag, p.err))) break;
       tc_fence_after();
       const uint32_t d = tmem + (static_cast<uint32_t>(qd * 32) << 16) + acc * kAccCols + part * kTileCols;
@@ -772,63 +773,95 @@ __global__ void __launch_bounds__(kMxThreads, 1)
       if (!mine) {
       } else if (it.phase == 1) {
         // 16 routes at a time, in pairs: a feature's gate lane takes the even one, its
-        // up lane the odd one, each handing the other the value it needs.  The scale
-        // of 32 features is two warps': they exchange exponents, by turns in two
-        // places, so that one barrier does.
+        // up lane the odd one, each handing the other the value it needs: eight
+        // activations of one feature a lane.
+        const int f = lane & 15, odd = lane >> 4;
+        // byte selectors of the 4 x 4 transposes below
+        const uint32_t swap1 = f & 1 ? 0x3715u : 0x6240u, swap2 = f & 2 ? 0x3276u : 0x5410u;
+        uint8_t* const to = p.act + (static_cast<int64_t>(it.start) + 2 * (f & 3) + odd) * (2 * p.inter) +
+                            tile * kMxFeatures + qd * 16 + (f & ~3);
+        uint8_t* const sb = p.as + (static_cast<int64_t>(it.start) + 2 * (f & 7) + odd) * p.pitch2 + tile * 2 + (qd >> 1);
         for (int c0 = 0; c0 < it.count; c0 += 16, turn ^= 1) {
           float v[16], a[8];
-          uint32_t top[8], h[4], l[4];
-          columns(c0, v);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float other = __shfl_xor_sync(0xffffffffu, low ? v[2 * j + 1] : v[2 * j], 16);
-            const float gate = low ? v[2 * j] : other, up = low ? other : v[2 * j + 1];
-            a[j] = __fdividef(gate, 1.0f + __expf(-gate)) * up;
-          }
-          uint8_t* ex = xchg + turn * 64;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const uint32_t e = (__float_as_uint(a[j]) >> 23) & 255u;
-            const uint32_t even = __reduce_max_sync(0xffffffffu, low ? e : 0u);
-            const uint32_t odd = __reduce_max_sync(0xffffffffu, low ? 0u : e);
-            top[j] = low ? even : odd;
-            if ((lane & 15) == 0) ex[qd * 16 + 2 * j + (lane >> 4)] = static_cast<uint8_t>(top[j]);
-          }
-          mx_epilogue_sync(bar);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            top[j] = max(top[j], static_cast<uint32_t>(ex[(qd ^ 1) * 16 + 2 * j + (lane >> 4)]));
-            top[j] = mx_block_byte(top[j]);
-            a[j] *= mx_block_mult(top[j]);
-          }
-#pragma unroll
-          for (int j = 0; j < 4; ++j) mx_split2(a[2 * j], a[2 * j + 1], &h[j], &l[j]);
-          const int first = c0 + (lane >> 4);
-          uint8_t* to = p.act + static_cast<int64_t>(it.start + first) * (2 * p.inter) +
-                        tile * kMxFeatures + qd * 16 + (lane & 15);
-          uint8_t* sb = p.as + static_cast<int64_t>(it.start + first) * p.pitch2 + tile * 2 + (qd >> 1);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            if (first + 2 * j < it.count) {
-              to[0] = static_cast<uint8_t>(j & 1 ? h[j / 2] >> 8 : h[j / 2]);
-              to[p.inter] = static_cast<uint8_t>(j & 1 ? l[j / 2] >> 8 : l[j / 2]);
-              if ((lane & 15) == 0 && (qd & 1) == 0) sb[0] = static_cast<uint8_t>(top[j]);
-            }
-            to += 4 * p.inter;
-            sb += 2 * p.pitch2;
-          }
-        }
-      } else {
-        __nv_bfloat16* to = p.out + static_cast<int64_t>(it.start) * p.hidden + tile * kMxM + qd * 32 + lane;
-        for (int c0 = 0; c0 < it.count; c0 += 16) {
-          float v[16];
+          uint32_t m[4], hi[2], lo[2];
           columns(c0, v);
           const float ws = c0 < 32 ? w[0] : c0 < 64 ? w[1] : c0 < 96 ? w[2] : w[3];
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float wj = __shfl_sync(0xffffffffu, ws, (c0 & 16) + j);
-            if (c0 + j < it.count) *to = __float2bfloat16_rn(v[j] * wj);
-            to += p.hidden;
+          for (int j = 0; j < 8; ++j) {
+            const float own = low ? v[2 * j] : v[2 * j + 1];
+            const float other = __shfl_xor_sync(0xffffffffu, low ? v[2 * j + 1] : v[2 * j], 16);
+            const float gate = low ? own : other, up = low ? other : own;
+            a[j] = __fdividef(gate, 1.0f + __expf(-gate)) * up *
+                   __shfl_sync(0xffffffffu, ws, (c0 & 16) + 2 * j + odd);
+          }
+          // The scale of 32 features is two warps'.  Largest magnitudes (their upper 16
+          // bits, two routes a register) of the warp's 16 features: a butterfly in which
+          // a lane keeps two registers, then one; then exchanged with the other warp, by
+          // turns in two places, so that one barrier does.
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            m[i] = __byte_perm(__float_as_uint(a[2 * i]), __float_as_uint(a[2 * i + 1]), 0x7632) & 0x7fff7fffu;
+          const bool b0 = f & 1, b1 = f & 2;
+          uint32_t k0 = __vmaxu2(b0 ? m[2] : m[0], __shfl_xor_sync(0xffffffffu, b0 ? m[0] : m[2], 1));
+          const uint32_t k1 = __vmaxu2(b0 ? m[3] : m[1], __shfl_xor_sync(0xffffffffu, b0 ? m[1] : m[3], 1));
+          k0 = __vmaxu2(b1 ? k1 : k0, __shfl_xor_sync(0xffffffffu, b1 ? k0 : k1, 2));
+          k0 = __vmaxu2(k0, __shfl_xor_sync(0xffffffffu, k0, 4));
+          k0 = __vmaxu2(k0, __shfl_xor_sync(0xffffffffu, k0, 8));
+          uint8_t* ex = xchg + turn * (4 * 32) + odd * 16;  // [warp][odd][route] of 16 bits
+          if (f < 4) *reinterpret_cast<uint32_t*>(ex + qd * 32 + ((f & 1) * 2 + (f >> 1)) * 4) = k0;
+          mx_epilogue_sync(bar);
+          const uint4 e0 = *reinterpret_cast<const uint4*>(ex + qd * 32);
+          const uint4 e1 = *reinterpret_cast<const uint4*>(ex + (qd ^ 1) * 32);
+          m[0] = __vmaxu2(e0.x, e1.x);
+          m[1] = __vmaxu2(e0.y, e1.y);
+          m[2] = __vmaxu2(e0.z, e1.z);
+          m[3] = __vmaxu2(e0.w, e1.w);
+          // times 2^(127 - byte), byte = max(exponent field - 7, 4); what a block that is
+          // not finite (byte 255) holds does not matter
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t z = __vminu2(0x01050105u - ((m[i] >> 7) & 0x00ff00ffu), 0x00fa00fau);
+            uint32_t h, l;
+            mx_split2(a[2 * i] * __uint_as_float(z << 23), a[2 * i + 1] * __uint_as_float((z & 0x00ff0000u) << 7),
+                      &h, &l);
+            hi[i / 2] = i & 1 ? hi[i / 2] | h << 16 : h;
+            lo[i / 2] = i & 1 ? lo[i / 2] | l << 16 : l;
+          }
+          // four routes of one feature -> four features of one route
+          auto transpose = [&](uint32_t x) {
+            x = __byte_perm(x, __shfl_xor_sync(0xffffffffu, x, 1), swap1);
+            return __byte_perm(x, __shfl_xor_sync(0xffffffffu, x, 2), swap2);
+          };
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            hi[i] = transpose(hi[i]);
+            lo[i] = transpose(lo[i]);
+            if (c0 + 8 * i + 2 * (f & 3) + odd < it.count) {
+              uint8_t* at = to + static_cast<int64_t>(c0 + 8 * i) * (2 * p.inter);
+              *reinterpret_cast<uint32_t*>(at) = hi[i];
+              *reinterpret_cast<uint32_t*>(at + p.inter) = lo[i];
+            }
+          }
+          if ((qd & 1) == 0 && f < 8 && c0 + 2 * f + odd < it.count) {
+            const uint32_t top = max(*reinterpret_cast<const uint16_t*>(ex + qd * 32 + f * 2),
+                                     *reinterpret_cast<const uint16_t*>(ex + (qd ^ 1) * 32 + f * 2));
+            sb[static_cast<int64_t>(c0) * p.pitch2] = static_cast<uint8_t>(mx_block_byte(top >> 7));
+          }
+        }
+      } else {
+        // 16 routes at a time, in pairs: an even lane takes the first one's two
+        // neighbouring features, an odd lane the second one's
+        const bool odd = lane & 1;
+        __nv_bfloat16* to = p.out + static_cast<int64_t>(it.start + odd) * p.hidden + tile * kMxM + qd * 32 + (lane & ~1);
+        for (int c0 = 0; c0 < it.count; c0 += 16) {
+          float v[16];
+          columns(c0, v);
+#pragma unroll
+          for (int j = 0; j < 16; j += 2) {
+            const float other = __shfl_xor_sync(0xffffffffu, odd ? v[j] : v[j + 1], 1);
+            const __nv_bfloat162 y = odd ? __floats2bfloat162_rn(other, v[j + 1]) : __floats2bfloat162_rn(v[j], other);
+            if (c0 + j + odd < it.count) *reinterpret_cast<__nv_bfloat162*>(to) = y;
+            to += 2 * p.hidden;
           }
         }
       }
