@@ -14,10 +14,16 @@
 //   equal groups) go to the lower id
 //   w = s[selected] (without the bias), / their sum if asked, * scaling
 //
-// The keys are formed and compared in 64 bits: two scores that 32 bits cannot
-// tell apart are common (a 16k-token batch has them in every call), and the
-// choice between them must not depend on the rounding of one exp.  Weights
-// are rounded once, at the store.
+// Keys are compared as 64-bit arithmetic orders them: two scores that 32 bits
+// cannot tell apart are common (a 16k-token batch has them in every call), and the
+// choice between them must not depend on the rounding of one exp.  But most tokens
+// have no such pair where it matters, and 64-bit exps cost five times all the rest.
+// So a token is first routed in 32 bits, with a bound on the keys' errors: if the
+// kept groups lie further from the dropped ones than the bound, and every selected
+// key further from the next one (or the two are exact ties: same logit, same bias),
+// the 64-bit order is the same.  Else (about 1 token in 100 with float32 logits) the
+// warp routes it once more in 64 bits.  Weights are rounded once, at the store;
+// float32 weights come from 64-bit values.
 //
 // One warp per token, no shared memory.  A group's experts lie in consecutive
 // lanes (lpg = the power of two <= 32 / G lanes per group, PER consecutive
@@ -40,6 +46,8 @@ struct RouteArgs {
   void* weights;      // [tokens, topk]
   int weights_type;   // FERRYB_BF16 / FP16 / FP32
   int top2, norm;
+  int quick;  // try 32 bits first
+  int whole;  // every lane of a group has `per` = PER experts, rows and bias aligned for wide loads
   float scaling;
 };
 
@@ -68,6 +76,267 @@ __device__ __forceinline__ double score_of(double l, double m, double z) {
 
 constexpr int kRouteWarps = 4;
 
+// ---- 32 bits ----
+// Order of floats that are not NaN as unsigned integers, 0 left for "not a
+// candidate", and back.
+__device__ __forceinline__ uint32_t order_of(float x) {
+  const uint32_t b = __float_as_uint(x + 0.0f);
+  return (b >> 31) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ float from_order(uint32_t k) {
+  return __uint_as_float((k >> 31) ? k & 0x7fffffffu : ~k);
+}
+
+// PER adjacent values as float, by the widest loads that fit (aligned to them).
+template <typename T, int PER>
+__device__ __forceinline__ void load_row(const T* p, float* v) {
+  constexpr int kBytes = PER * sizeof(T), kVec = kBytes < 16 ? kBytes : 16, kEach = kVec / sizeof(T);
+#pragma unroll
+  for (int i = 0; i < PER; i += kEach) {
+    alignas(16) T x[kEach];
+    if (kVec == 16) *reinterpret_cast<uint4*>(x) = *reinterpret_cast<const uint4*>(p + i);
+    else *reinterpret_cast<uint2*>(x) = *reinterpret_cast<const uint2*>(p + i);
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) v[i + j] = static_cast<float>(x[j]);
+  }
+}
+
+// exp to about 2^-31: x = n ln 2 + r, |r| <= ln 2 / 2, Taylor's polynomial of degree
+// 9 for exp(r) (remainder below 0.347^10 / 10! = 2^-37), exponent set by hand.
+// For |x| <= 700.
+__device__ __forceinline__ double exp_f64(double x) {
+  const float n = rintf(static_cast<float>(x) * 1.4426950408889634f);
+  const double r = fma(static_cast<double>(-n), 0.693147180559945309417, x);
+  double y = 1.0 / 362880;
+  y = fma(y, r, 1.0 / 40320);
+  y = fma(y, r, 1.0 / 5040);
+  y = fma(y, r, 1.0 / 720);
+  y = fma(y, r, 1.0 / 120);
+  y = fma(y, r, 1.0 / 24);
+  y = fma(y, r, 1.0 / 6);
+  y = fma(y, r, 0.5);
+  y = fma(y, r, 1.0);
+  y = fma(y, r, 1.0);
+  return y * __hiloint2double((1023 + static_cast<int>(n)) << 20, 0);
+}
+// 1 / x for x in the range of float: the float reciprocal (2^-23) and a Newton step.
+__device__ __forceinline__ double rcp_f64(double x) {
+  const double y = static_cast<double>(__frcp_rn(static_cast<float>(x)));
+  return fma(y, fma(-x, y, 1.0), y);
+}
+
+__device__ __forceinline__ void store_weight(const RouteArgs& a, int64_t at, double w) {
+  if (a.weights_type == FERRYB_FP32) static_cast<float*>(a.weights)[at] = static_cast<float>(w);
+  else if (a.weights_type == FERRYB_FP16) static_cast<__half*>(a.weights)[at] = __double2half(w);
+  else static_cast<__nv_bfloat16*>(a.weights)[at] = __double2bfloat16(w);
+}
+__device__ __forceinline__ void store_weight(const RouteArgs& a, int64_t at, float w) {
+  if (a.weights_type == FERRYB_FP32) static_cast<float*>(a.weights)[at] = w;
+  else if (a.weights_type == FERRYB_FP16) static_cast<__half*>(a.weights)[at] = __float2half_rn(w);
+  else static_cast<__nv_bfloat16*>(a.weights)[at] = __float2bfloat16_rn(w);
+}
+
+// Errors of float32 scores, in units of 2^-24 of them and generously.
+// Softmax: __expf(-x) has 4 + 2.4 x (its documented bound) and x for the rounding of
+// its argument; the sum the mean of that under softmax (the mean of x is at most
+// ln 1024 = 7) and 37 for its additions; reciprocal and product 4: 75 + 3.4 x.  Times
+// the score that falls with x, so two scores, the larger one k at x, may be taken as
+// ordered if they lie 2 (75 + 3.4 x) k apart; without x, 2 (75 + 3.4 * 88) k.
+// Sigmoid: (1 - s) (4 + 2.4 |l|) from exp(-l), 5 for sum and quotient; that is s (4 +
+// 2.4 * 88 + 5) at most, and 7 against a score of 1.
+// The key sort below drops the lowest bits of a key: 2^kBits of its units.
+constexpr float kUnit = 1.0f / (1 << 24);
+constexpr float kFar = 80.0f;  // scores further than e^-80 from the largest are left to 64 bits
+
+// True if the token's routing is certain, and stored.
+template <typename T, int PER, bool SOFTMAX>
+__device__ __forceinline__ bool route_quick(const RouteArgs& a, int64_t t, int lane, const T* row, int group,
+                                            int first, int mine) {
+  constexpr uint32_t kAll = 0xffffffffu;
+  constexpr int kBits = PER == 4 ? 2 : PER == 8 ? 3 : PER == 16 ? 4 : 5;
+  constexpr uint32_t kIndex = (1u << kBits) - 1;
+  float v[PER];
+  if (a.whole) {
+    if (mine > 0) load_row<T, PER>(row + first, v);
+    else {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) v[i] = -CUDART_INF_F;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) v[i] = i < mine ? static_cast<float>(row[first + i]) : -CUDART_INF_F;
+  }
+  float m = -CUDART_INF_F, z = 0.0f, largest = 1.0f;
+  if (SOFTMAX) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) m = fmaxf(m, v[i]);
+    m = from_order(__reduce_max_sync(kAll, order_of(m)));
+    if (!(fabsf(m) < CUDART_INF_F)) return false;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) { v[i] = __expf(v[i] - m); z += v[i]; }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(kAll, z, o);
+    if (z != z) return false;  // a NaN among the logits
+    largest = __frcp_rn(z);  // the score of the largest logit
+#pragma unroll
+    for (int i = 0; i < PER; ++i) v[i] *= largest;
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) v[i] = __fdividef(1.0f, 1.0f + __expf(-v[i]));
+  }
+  if (a.bias) {
+    if (a.whole) {
+      float bias[PER];
+      if (mine > 0) {
+        load_row<float, PER>(a.bias + first, bias);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) v[i] += bias[i];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) if (i < mine) v[i] += a.bias[first + i];
+    }
+  }
+  if (!SOFTMAX || a.bias) {
+    float sum = 0.0f;  // not a number if a key is not
+#pragma unroll
+    for (int i = 0; i < PER; ++i) sum += v[i];
+    if (__any_sync(kAll, sum != sum)) return false;
+  }
+  // how far two keys must lie apart, the larger one being k
+  auto gap = [&](float k, float x) {
+    const float cut = 2.0f * (kIndex + 2) * fabsf(k);
+    if (a.bias) return kUnit * ((SOFTMAX ? 160.0f : 16.0f) * largest + cut);
+    return kUnit * ((SOFTMAX ? 150.0f + 7.0f * x : 512.0f) * k + cut);
+  };
+  if (a.groups > 1) {
+    float best = -CUDART_INF_F, second = -CUDART_INF_F;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const float k = i < mine ? v[i] : -CUDART_INF_F;
+      second = fmaxf(second, fminf(best, k));
+      best = fmaxf(best, k);
+    }
+    for (int o = 1; o < a.lpg; o <<= 1) {
+      const float ob = __shfl_xor_sync(kAll, best, o), os = __shfl_xor_sync(kAll, second, o);
+      second = fmaxf(fminf(best, ob), fmaxf(second, os));
+      best = fmaxf(best, ob);
+    }
+    const uint32_t worth = order_of(a.top2 ? best + second : best);
+    int rank = 0;
+    for (int g = 0; g < a.groups; ++g) {
+      const uint32_t w = __shfl_sync(kAll, worth, g * a.lpg);
+      rank += w > worth || (w == worth && g < group);
+    }
+    const bool stays = rank < a.kept;
+    if (a.kept < a.groups) {
+      const bool real = group < a.groups;
+      const float in = from_order(__reduce_min_sync(kAll, real && stays ? worth : 0xffffffffu));
+      const float out = from_order(__reduce_max_sync(kAll, real && !stays ? worth : 0u));
+      if (!(in - out > 2.0f * gap(in, 88.0f))) return false;  // a sum of two has both errors
+    }
+    if (!stays) mine = 0;
+  }
+  // A lane's keys in descending order, the place of each in the bits that it loses:
+  // of equal keys the lower id comes first, in a lane and, as the heads are compared
+  // without those bits, among lanes.
+  uint32_t key[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) key[i] = i < mine ? (order_of(v[i]) & ~kIndex) | (kIndex - i) : 0u;
+  // Batcher's odd-even mergesort
+#pragma unroll
+  for (int p = 1; p < PER; p *= 2) {
+#pragma unroll
+    for (int q = p; q >= 1; q /= 2) {
+#pragma unroll
+      for (int j = q % p; j + q < PER; j += 2 * q) {
+#pragma unroll
+        for (int i = 0; i < q; ++i) {
+          if (i + j + q < PER && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
+            const uint32_t x = key[i + j], y = key[i + j + q];
+            key[i + j] = max(x, y);
+            key[i + j + q] = min(x, y);
+          }
+        }
+      }
+    }
+  }
+  // the largest key left, and its expert
+  auto take = [&](uint32_t* top) {
+    const uint32_t head = key[0] | kIndex;  // (kIndex where nothing is left)
+    *top = __reduce_max_sync(kAll, head);
+    const int winner = __ffs(__ballot_sync(kAll, head == *top)) - 1;
+    const int id = __shfl_sync(kAll, first + static_cast<int>(kIndex - (key[0] & kIndex)), winner);
+    if (lane == winner) {
+#pragma unroll
+      for (int i = 0; i + 1 < PER; ++i) key[i] = key[i + 1];
+      key[PER - 1] = 0;
+    }
+    return id;
+  };
+  int chosen = 0;
+  uint32_t chosen_key = 0, top;
+  for (int j = 0; j < a.topk; ++j) {
+    const int id = take(&top);
+    if (lane == j) { chosen = id; chosen_key = top; }
+  }
+  const bool holds = lane < a.topk;
+  const float l = holds ? static_cast<float>(row[chosen]) : 0.0f;
+  const float bias = holds && a.bias ? a.bias[chosen] : 0.0f;
+  const float k = from_order(chosen_key);
+  {
+    const float k1 = __shfl_down_sync(kAll, k, 1), l1 = __shfl_down_sync(kAll, l, 1);
+    const float b1 = __shfl_down_sync(kAll, bias, 1);
+    bool sure = lane + 1 >= a.topk || k - k1 > gap(k, m - l) || (l == l1 && bias == b1);
+    // scores near the end of float's range, and weights of them
+    sure &= !holds || (SOFTMAX ? l - m > -kFar : l > -kFar);
+    if (!__all_sync(kAll, sure)) return false;
+  }
+  // the first key that is left out: further away, or an exact tie (of a higher id)
+  // and then the next one
+  {
+    const float last = __shfl_sync(kAll, k, a.topk - 1), last_l = __shfl_sync(kAll, l, a.topk - 1);
+    const float last_b = __shfl_sync(kAll, bias, a.topk - 1), apart = gap(last, m - last_l);
+    for (;;) {
+      const int id = take(&top);
+      if (top == kIndex || last - from_order(top) > apart) break;
+      if (static_cast<float>(row[id]) != last_l || (a.bias && a.bias[id] != last_b)) return false;
+    }
+  }
+  const int64_t o = t * a.topk + lane;
+  if (a.weights_type == FERRYB_FP32) {
+    // without `norm` only sigmoid scores come here
+    double w = holds ? (SOFTMAX ? exp_f64(static_cast<double>(l) - static_cast<double>(m))
+                                : rcp_f64(1.0 + exp_f64(fmax(-static_cast<double>(l), -700.0))))
+                     : 0.0;
+    if (a.norm) {
+      double sum = w;
+#pragma unroll
+      for (int i = 16; i > 0; i >>= 1) sum += shfl_xor_f64(sum, i);
+      w *= rcp_f64(sum);
+    }
+    if (holds) {
+      a.selected[o] = chosen;
+      store_weight(a, o, w * static_cast<double>(a.scaling));
+    }
+  } else {
+    float w = holds ? (SOFTMAX ? expf(l - m) : __frcp_rn(1.0f + expf(-l))) : 0.0f;
+    if (a.norm) {
+      float sum = w;
+#pragma unroll
+      for (int i = 16; i > 0; i >>= 1) sum += __shfl_xor_sync(kAll, sum, i);
+      w /= sum;
+    } else if (SOFTMAX) {
+      w *= largest;
+    }
+    if (holds) {
+      a.selected[o] = chosen;
+      store_weight(a, o, w * a.scaling);
+    }
+  }
+  return true;
+}
+
 template <typename T, int PER, bool SOFTMAX>
 __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RouteArgs a) {
   const int64_t t = static_cast<int64_t>(blockIdx.x) * kRouteWarps + (threadIdx.x >> 5);
@@ -77,7 +346,9 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RouteArgs
   const int group = lane / a.lpg, in_group = (lane % a.lpg) * a.per;
   const int first = group * a.gsize + in_group;
   const int mine = group < a.groups ? min(a.per, a.gsize - in_group) : 0;  // may be <= 0
+  if (a.quick && route_quick<T, PER, SOFTMAX>(a, t, lane, row, group, first, mine)) return;
 
+  // ---- 64 bits ----
   double v[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) v[i] = i < mine ? load_f64(row + first + i) : -CUDART_INF;
@@ -170,20 +441,27 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RouteArgs
     w *= static_cast<double>(a.scaling);
     const int64_t o = t * a.topk + lane;
     a.selected[o] = chosen;
-    if (a.weights_type == FERRYB_FP32) static_cast<float*>(a.weights)[o] = static_cast<float>(w);
-    else if (a.weights_type == FERRYB_FP16) static_cast<__half*>(a.weights)[o] = __double2half(w);
-    else static_cast<__nv_bfloat16*>(a.weights)[o] = __double2bfloat16(w);
+    store_weight(a, o, w);
   }
 }
 
+template <typename T, int PER, bool SOFTMAX>
+static void route_launch(RouteArgs a, cudaStream_t stream) {
+  const unsigned grid = static_cast<unsigned>((a.tokens + kRouteWarps - 1) / kRouteWarps);
+  constexpr uintptr_t kVec = PER * sizeof(T) < 16 ? PER * sizeof(T) : 16;
+  a.whole = a.per == PER && a.gsize == a.lpg * PER && reinterpret_cast<uintptr_t>(a.logits) % kVec == 0 &&
+            (a.tokens <= 1 || a.row_stride * sizeof(T) % kVec == 0) &&
+            reinterpret_cast<uintptr_t>(a.bias) % 16 == 0;
+  // float32 softmax weights that are not renormalised need the sum in 64 bits
+  a.quick = !(SOFTMAX && !a.norm && a.weights_type == FERRYB_FP32);
+  route_kernel<T, PER, SOFTMAX><<<grid, kRouteWarps * 32, 0, stream>>>(a);
+}
 template <typename T, bool SOFTMAX>
 static int route_per(const RouteArgs& a, cudaStream_t stream) {
-  const unsigned grid = static_cast<unsigned>((a.tokens + kRouteWarps - 1) / kRouteWarps);
-  constexpr int kT = kRouteWarps * 32;
-  if (a.per <= 4) route_kernel<T, 4, SOFTMAX><<<grid, kT, 0, stream>>>(a);
-  else if (a.per <= 8) route_kernel<T, 8, SOFTMAX><<<grid, kT, 0, stream>>>(a);
-  else if (a.per <= 16) route_kernel<T, 16, SOFTMAX><<<grid, kT, 0, stream>>>(a);
-  else route_kernel<T, 32, SOFTMAX><<<grid, kT, 0, stream>>>(a);
+  if (a.per <= 4) route_launch<T, 4, SOFTMAX>(a, stream);
+  else if (a.per <= 8) route_launch<T, 8, SOFTMAX>(a, stream);
+  else if (a.per <= 16) route_launch<T, 16, SOFTMAX>(a, stream);
+  else route_launch<T, 32, SOFTMAX>(a, stream);
   FB_LAUNCH_CHECK();
   return FERRYB_OK;
 }
