@@ -13,6 +13,7 @@ workspace, and neither copy to the host nor wait for the GPU, so they can be
 captured into a CUDA graph.
 """
 import ctypes
+import functools
 
 import torch
 
@@ -140,8 +141,9 @@ def scatter_returned(returned, send_idx, tokens):
 def _cuda_call(device, name, *args):
     """call() on `device`'s current stream, whatever the current device is."""
     # the raw stream costs a tenth of a microsecond, a torch.cuda.Stream three
-    stream = torch._C._cuda_getCurrentRawStream(device.index)
-    if device.index == torch.cuda.current_device():
+    index = device.index
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if index == torch._C._cuda_getDevice():
         call(name, *args, stream)
     else:
         with torch.cuda.device(device):
@@ -263,9 +265,12 @@ def quantize_mxfp4(x, out=None):
     if x.numel() == 0:
         return codes, scales
     x2 = _dense_rows(x if x.dim() == 2 else x.reshape(-1, width))
-    c2, s2 = _rows_2d(codes, 'codes'), _rows_2d(scales, 'scales')
+    code_stride, scale_stride = width // 2, width // 32
+    if out is not None:
+        code_stride = _rows_2d(codes, 'codes').stride(0)
+        scale_stride = _rows_2d(scales, 'scales').stride(0)
     _cuda_call(x.device, 'ferryb_quantize_mxfp4', x2.data_ptr(), kind, x2.shape[0], width, x2.stride(0),
-               c2.data_ptr(), c2.stride(0), s2.data_ptr(), s2.stride(0))
+               codes.data_ptr(), code_stride, scales.data_ptr(), scale_stride)
     return codes, scales
 
 
@@ -284,17 +289,27 @@ def dequantize_mxfp4(codes, scales, dtype=BF16, out=None):
     if kind is None:
         raise _lib.FerrybError('dtype must be bf16, fp16 or float32')
     _same_device(codes.device, scales=scales, out=out)
+    out_stride = width
     if out is None:
         out = codes.new_empty((*lead, width), dtype=dtype)
     elif out.dtype != dtype or out.shape != (*lead, width):
         raise _lib.FerrybError(f'out must be {dtype} {[*lead, width]}')
+    else:
+        out_stride = _rows_2d(out, 'out').stride(0) if out.numel() else 0
     if out.numel() == 0:
         return out
-    o2 = _rows_2d(out, 'out')
     c2, s2 = (_dense_rows(t if t.dim() == 2 else t.reshape(-1, t.shape[-1])) for t in (codes, scales))
     _cuda_call(codes.device, 'ferryb_dequantize_mxfp4', c2.data_ptr(), c2.stride(0), s2.data_ptr(), s2.stride(0),
-               o2.shape[0], width, o2.data_ptr(), kind, o2.stride(0))
+               c2.shape[0], width, out.data_ptr(), kind, out_stride)
     return out
+
+
+@functools.lru_cache(maxsize=256)
+def _mxfp4_workspace(routes, groups, hidden, intermediate):
+    size = _lib.lib().ferryb_execute_experts_mxfp4_workspace(routes, groups, hidden, intermediate)
+    if size < 0:
+        raise _lib.FerrybError(_lib.lib().ferryb_last_error().decode())
+    return size
 
 
 def execute_experts_mxfp4(cache, input, routing_weights, slots, starts, rows, cols, hidden, intermediate,
@@ -318,9 +333,11 @@ def execute_experts_mxfp4(cache, input, routing_weights, slots, starts, rows, co
     that starts at 0, it returns at once and leaves a non-zero code there for
     the caller to check, and can be captured into a CUDA graph."""
     require_cuda(cache, input, routing_weights, slots, starts, rows, cols, out, err)
-    dev = input.device
-    _same_device(dev, cache=cache, routing_weights=routing_weights, slots=slots, starts=starts, rows=rows,
-                 cols=cols, out=out, err=err)
+    dev, index = input.device, input.get_device()
+    for t in (cache, routing_weights, slots, starts, rows, cols, out, err):
+        if t is not None and t.get_device() != index:
+            _same_device(dev, cache=cache, routing_weights=routing_weights, slots=slots, starts=starts,
+                         rows=rows, cols=cols, out=out, err=err)
     hidden, intermediate = int(hidden), int(intermediate)
     if hidden <= 0 or intermediate <= 0 or hidden % 128 or intermediate % 128:
         raise _lib.FerrybError(f'hidden ({hidden}) and intermediate ({intermediate}) must be multiples of 128')
@@ -334,9 +351,9 @@ def execute_experts_mxfp4(cache, input, routing_weights, slots, starts, rows, co
     weights_type = _lib.ELEMENT_TYPES.get(routing_weights.dtype)
     if weights_type is None or routing_weights.dim() != 2 or routing_weights.shape[0] != tokens:
         raise _lib.FerrybError('routing_weights must be bf16, fp16 or float32 [n, topk]')
-    for name, t in (('slots', slots), ('starts', starts), ('rows', rows), ('cols', cols)):
+    for t in (slots, starts, rows, cols):
         if t.dtype != torch.int64 or t.dim() != 1:
-            raise _lib.FerrybError(f'{name} must be a 1-D int64 tensor')
+            raise _lib.FerrybError('slots, starts, rows and cols must be 1-D int64 tensors')
     groups, routes = slots.shape[0], rows.shape[0]
     if starts.shape[0] != groups + 1:
         raise _lib.FerrybError(f'starts must have {groups + 1} entries (one more than slots)')
@@ -357,9 +374,7 @@ def execute_experts_mxfp4(cache, input, routing_weights, slots, starts, rows, co
         stride = hidden
     routing_weights = routing_weights.contiguous()
     slots, starts, rows, cols = slots.contiguous(), starts.contiguous(), rows.contiguous(), cols.contiguous()
-    ws_bytes = _lib.lib().ferryb_execute_experts_mxfp4_workspace(routes, groups, hidden, intermediate)
-    if ws_bytes < 0:
-        raise _lib.FerrybError(_lib.lib().ferryb_last_error().decode())
+    ws_bytes = _mxfp4_workspace(routes, groups, hidden, intermediate)
     ws = cache.new_empty((ws_bytes,))
     if wait:
         err = torch.zeros(1, dtype=torch.int32, device=dev)
