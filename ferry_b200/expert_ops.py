@@ -14,6 +14,7 @@ captured into a CUDA graph.
 """
 import ctypes
 import functools
+import struct
 
 import torch
 
@@ -159,6 +160,8 @@ def _same_device(device, **tensors):
 def _dense_rows(t):
     """2-D t itself if the values of a row are adjacent and its rows do not
     overlap, else a contiguous copy."""
+    if t.is_contiguous():
+        return t
     rows, width = t.shape
     stride, step = t.stride()
     return t if (step == 1 or width <= 1) and (stride >= width or rows <= 1) else t.contiguous()
@@ -206,11 +209,15 @@ def route_experts(logits, topk, *, score='softmax', bias=None, n_group=1, topk_g
         raise _lib.FerrybError(f'topk must be in [1, {experts}]')
     selected = logits.new_empty((tokens, topk), dtype=torch.int64)
     weights = logits.new_empty((tokens, topk), dtype=weights_dtype)
-    args = _lib.RouteArgs(logits.data_ptr(), tokens, logits.stride(0), experts, topk, int(n_group),
-                          int(topk_group), logits_type, weights_type, SCORES[score], GROUP_SCORES[group_score],
-                          int(bool(norm_topk_prob)), float(scaling), _lib.addr(bias),
-                          selected.data_ptr(), weights.data_ptr())
-    _cuda_call(dev, 'ferryb_route_experts', ctypes.byref(args))
+    try:
+        args = _lib.pack_route_args(
+            logits.data_ptr(), tokens, logits.stride(0), experts, topk, int(n_group), int(topk_group), logits_type,
+            weights_type, SCORES[score], GROUP_SCORES[group_score], int(bool(norm_topk_prob)), float(scaling),
+            _lib.addr(bias), selected.data_ptr(), weights.data_ptr())
+    except (struct.error, OverflowError):
+        raise _lib.FerrybError(f'n_group ({n_group}), topk_group ({topk_group}) or scaling ({scaling}) is too '
+                               'large') from None
+    _cuda_call(dev, 'ferryb_route_experts', args)
     return selected, weights
 
 
@@ -378,11 +385,11 @@ def execute_experts_mxfp4(cache, input, routing_weights, slots, starts, rows, co
     ws = cache.new_empty((ws_bytes,))
     if wait:
         err = torch.zeros(1, dtype=torch.int32, device=dev)
-    args = _lib.Mxfp4ExpertsArgs(
+    args = _lib.pack_mxfp4_experts_args(
         cache.data_ptr(), cache.shape[0], input.data_ptr(), tokens, stride, routing_weights.data_ptr(),
         routing_weights.shape[1], weights_type, 0, slots.data_ptr(), starts.data_ptr(), groups, rows.data_ptr(),
         cols.data_ptr(), routes, hidden, intermediate, out.data_ptr(), ws.data_ptr(), ws_bytes, err.data_ptr())
-    _cuda_call(dev, 'ferryb_execute_experts_mxfp4', ctypes.byref(args))
+    _cuda_call(dev, 'ferryb_execute_experts_mxfp4', args)
     if wait:
         _lib.check_device_error(err, 'execute_experts_mxfp4')
     return out

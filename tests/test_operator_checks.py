@@ -35,7 +35,7 @@ def test_route_checks(calls):
     assert sel.shape == w.shape == (3, 2) and w.dtype == BF16 and len(calls) == 1
     for bad in (dict(logits=x.double()), dict(logits=x[0]), dict(topk=0), dict(topk=9), dict(score='tanh'),
                 dict(group_score='sum'), dict(bias=torch.zeros(7)), dict(bias=torch.zeros(8, dtype=BF16)),
-                dict(weights_dtype=torch.float64)):
+                dict(weights_dtype=torch.float64), dict(n_group=2**40)):
         args = dict(logits=x, topk=2)
         args.update(bad)
         with pytest.raises(FerrybError):
