@@ -22,8 +22,9 @@
 // kept groups lie further from the dropped ones than the bound, and every selected
 // key further from the next one (or the two are exact ties: same logit, same bias),
 // the 64-bit order is the same.  Else (about 1 token in 100 with float32 logits) the
-// warp routes it once more in 64 bits.  Weights are rounded once, at the store;
-// float32 weights come from 64-bit values.
+// warp routes it once more in 64 bits.  Weights are formed in 64 bits in any case (of
+// the K selected only, and the sum where softmax weights are not renormalised) and
+// rounded once, at the store.
 //
 // One warp per token, no shared memory.  A group's experts lie in consecutive
 // lanes (lpg = the power of two <= 32 / G lanes per group, PER consecutive
@@ -46,7 +47,6 @@ struct RouteArgs {
   void* weights;      // [tokens, topk]
   int weights_type;   // FERRYB_BF16 / FP16 / FP32
   int top2, norm;
-  int quick;  // try 32 bits first
   int whole;  // every lane of a group has `per` = PER experts, rows and bias aligned for wide loads
   float scaling;
 };
@@ -101,13 +101,15 @@ __device__ __forceinline__ void load_row(const T* p, float* v) {
   }
 }
 
-// exp to about 2^-31: x = n ln 2 + r, |r| <= ln 2 / 2, Taylor's polynomial of degree
-// 9 for exp(r) (remainder below 0.347^10 / 10! = 2^-37), exponent set by hand.
-// For |x| <= 700.
+// exp to about 2^-46: x = n ln 2 + r, |r| <= ln 2 / 2, Taylor's polynomial of degree
+// 11 for exp(r) (remainder below 0.347^12 / 12! = 2^-47), exponent set by hand.
+// For |x| <= 700; a third of exp()'s instructions.
 __device__ __forceinline__ double exp_f64(double x) {
   const float n = rintf(static_cast<float>(x) * 1.4426950408889634f);
   const double r = fma(static_cast<double>(-n), 0.693147180559945309417, x);
-  double y = 1.0 / 362880;
+  double y = 1.0 / 39916800;
+  y = fma(y, r, 1.0 / 3628800);
+  y = fma(y, r, 1.0 / 362880);
   y = fma(y, r, 1.0 / 40320);
   y = fma(y, r, 1.0 / 5040);
   y = fma(y, r, 1.0 / 720);
@@ -130,12 +132,6 @@ __device__ __forceinline__ void store_weight(const RouteArgs& a, int64_t at, dou
   else if (a.weights_type == FERRYB_FP16) static_cast<__half*>(a.weights)[at] = __double2half(w);
   else static_cast<__nv_bfloat16*>(a.weights)[at] = __double2bfloat16(w);
 }
-__device__ __forceinline__ void store_weight(const RouteArgs& a, int64_t at, float w) {
-  if (a.weights_type == FERRYB_FP32) static_cast<float*>(a.weights)[at] = w;
-  else if (a.weights_type == FERRYB_FP16) static_cast<__half*>(a.weights)[at] = __float2half_rn(w);
-  else static_cast<__nv_bfloat16*>(a.weights)[at] = __float2bfloat16_rn(w);
-}
-
 // Errors of float32 scores, in units of 2^-24 of them and generously.
 // Softmax: __expf(-x) has 4 + 2.4 x (its documented bound) and x for the rounding of
 // its argument; the sum the mean of that under softmax (the mean of x is at most
@@ -152,6 +148,7 @@ constexpr float kFar = 80.0f;  // scores further than e^-80 from the largest are
 template <typename T, int PER, bool SOFTMAX>
 __device__ __forceinline__ bool route_quick(const RouteArgs& a, int64_t t, int lane, const T* row, int group,
                                             int first, int mine) {
+  const int all = mine;
   constexpr uint32_t kAll = 0xffffffffu;
   constexpr int kBits = PER == 4 ? 2 : PER == 8 ? 3 : PER == 16 ? 4 : 5;
   constexpr uint32_t kIndex = (1u << kBits) - 1;
@@ -304,35 +301,24 @@ __device__ __forceinline__ bool route_quick(const RouteArgs& a, int64_t t, int l
     }
   }
   const int64_t o = t * a.topk + lane;
-  if (a.weights_type == FERRYB_FP32) {
-    // without `norm` only sigmoid scores come here
-    double w = holds ? (SOFTMAX ? exp_f64(static_cast<double>(l) - static_cast<double>(m))
-                                : rcp_f64(1.0 + exp_f64(fmax(-static_cast<double>(l), -700.0))))
-                     : 0.0;
-    if (a.norm) {
-      double sum = w;
+  double w = 0.0, sum = 0.0;
+  if (holds)
+    w = SOFTMAX ? exp_f64(static_cast<double>(l) - static_cast<double>(m))
+                : rcp_f64(1.0 + exp_f64(fmax(-static_cast<double>(l), -700.0)));
+  if (a.norm) {
+    sum = w;
+  } else if (SOFTMAX) {
+    for (int i = 0; i < all; ++i)
+      sum += exp_f64(fmax(static_cast<double>(static_cast<float>(row[first + i])) - static_cast<double>(m), -700.0));
+  }
+  if (a.norm || SOFTMAX) {
 #pragma unroll
-      for (int i = 16; i > 0; i >>= 1) sum += shfl_xor_f64(sum, i);
-      w *= rcp_f64(sum);
-    }
-    if (holds) {
-      a.selected[o] = chosen;
-      store_weight(a, o, w * static_cast<double>(a.scaling));
-    }
-  } else {
-    float w = holds ? (SOFTMAX ? expf(l - m) : __frcp_rn(1.0f + expf(-l))) : 0.0f;
-    if (a.norm) {
-      float sum = w;
-#pragma unroll
-      for (int i = 16; i > 0; i >>= 1) sum += __shfl_xor_sync(kAll, sum, i);
-      w /= sum;
-    } else if (SOFTMAX) {
-      w *= largest;
-    }
-    if (holds) {
-      a.selected[o] = chosen;
-      store_weight(a, o, w * a.scaling);
-    }
+    for (int i = 16; i > 0; i >>= 1) sum += shfl_xor_f64(sum, i);
+    w *= rcp_f64(sum);
+  }
+  if (holds) {
+    a.selected[o] = chosen;
+    store_weight(a, o, w * static_cast<double>(a.scaling));
   }
   return true;
 }
@@ -346,7 +332,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RouteArgs
   const int group = lane / a.lpg, in_group = (lane % a.lpg) * a.per;
   const int first = group * a.gsize + in_group;
   const int mine = group < a.groups ? min(a.per, a.gsize - in_group) : 0;  // may be <= 0
-  if (a.quick && route_quick<T, PER, SOFTMAX>(a, t, lane, row, group, first, mine)) return;
+  if (route_quick<T, PER, SOFTMAX>(a, t, lane, row, group, first, mine)) return;
 
   // ---- 64 bits ----
   double v[PER];
@@ -452,8 +438,6 @@ static void route_launch(RouteArgs a, cudaStream_t stream) {
   a.whole = a.per == PER && a.gsize == a.lpg * PER && reinterpret_cast<uintptr_t>(a.logits) % kVec == 0 &&
             (a.tokens <= 1 || a.row_stride * sizeof(T) % kVec == 0) &&
             reinterpret_cast<uintptr_t>(a.bias) % 16 == 0;
-  // float32 softmax weights that are not renormalised need the sum in 64 bits
-  a.quick = !(SOFTMAX && !a.norm && a.weights_type == FERRYB_FP32);
   route_kernel<T, PER, SOFTMAX><<<grid, kRouteWarps * 32, 0, stream>>>(a);
 }
 template <typename T, bool SOFTMAX>

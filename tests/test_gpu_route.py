@@ -153,3 +153,35 @@ def test_feeds_the_runtime():
         want, _, _ = orc.execute(layer, [x], [sel.cpu()], [w.cpu()])
         assert_bf16_close(got.cpu(), want[0])
     rt.close()
+
+
+@pytest.mark.parametrize('score', ['softmax', 'sigmoid'])
+@pytest.mark.parametrize('groups,kept,group_score', [(1, 1, 'max'), (8, 3, 'max'), (8, 4, 'top2')])
+def test_close_keys(score, groups, kept, group_score):
+    """Keys a few to a few thousand units of float32 apart, with and without a
+    bias that brings different scores together: the 64-bit order decides."""
+    g = torch.Generator().manual_seed(groups)
+    kw = dict(score=score, n_group=groups, topk_group=kept, group_score=group_score)
+    for spread in (2.0 ** -24, 2.0 ** -21, 2.0 ** -18, 2.0 ** -14, 2.0 ** -10):
+        x = 1 + spread * torch.randint(-64, 64, (40, 128), generator=g).float()
+        _check(x, 8, **kw)
+        bias = torch.randn(128, generator=g)
+        score_of = torch.softmax if score == 'softmax' else (lambda t, d: torch.sigmoid(t))
+        y = torch.randn(1, 128, generator=g)
+        close = 3 - score_of(y.double(), 1)[0].float() + spread * torch.randint(-64, 64, (128,), generator=g).float()
+        _check(y.expand(3, 128).contiguous(), 8, bias=close, **kw)
+        _check(torch.randn(40, 128, generator=g), 8, bias=bias * spread, **kw)
+
+
+def test_ties_across_the_border():
+    """More equal logits than places, equal logits under different biases, and
+    scores far below the largest."""
+    x = torch.full((5, 128), -1.0)
+    x[1, 3::7] = 2.0
+    x[2, :4] = torch.tensor([5.0, 4.0, 3.0, 2.0])
+    x[3, 100:] = -100.0
+    x[4, 10:] = -200.0
+    for score in ('softmax', 'sigmoid'):
+        for topk in (1, 8, 17, 32):
+            _check(x, topk, score=score)
+            _check(x, topk, score=score, bias=torch.arange(128).remainder(3).float() * 0.25)
