@@ -167,6 +167,7 @@ SIGNATURES = {
 }
 
 _lib = None
+_fast = None
 
 
 class FerrybError(RuntimeError):
@@ -190,6 +191,35 @@ def lib():
             fn.restype, fn.argtypes = res, args
         _lib = handle
     return _lib
+
+
+class _NoFast:
+    """Stands in for the extension where it is not built: nothing is a plain case."""
+
+    @staticmethod
+    def _none(*args):
+        return None
+
+    route_experts = quantize_mxfp4 = dequantize_mxfp4 = execute_experts_mxfp4 = _none
+
+
+def fast():
+    """The _fast extension (csrc/expert_ops_fast.cpp), which answers the plain
+    cases of four operators and returns None for the rest."""
+    global _fast
+    if _fast is None:
+        try:
+            from . import _fast as module
+        except ImportError:
+            module = None
+        if module is None:
+            _fast = _NoFast
+        else:
+            module.init(*(ctypes.cast(getattr(lib(), name), ctypes.c_void_p).value for name in (
+                'ferryb_route_experts', 'ferryb_quantize_mxfp4', 'ferryb_dequantize_mxfp4',
+                'ferryb_execute_experts_mxfp4_workspace', 'ferryb_execute_experts_mxfp4')))
+            _fast = module
+    return _fast
 
 
 def call(name, *args):

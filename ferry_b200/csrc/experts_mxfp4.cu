@@ -16,35 +16,52 @@
 // parts are multiplied and summed into the same float32 accumulator.  A block's
 // largest value is brought to [2^7, 2^8); hi + lo is then the bf16 number itself
 // down to 2^-6 (2^-13 of the largest) and within 2^-14 (2^-21 of the largest)
-// below that, half the lo part's smallest step of 2^-9 * 2^-4.  The activation,
-// operand of the second product, is stored the same way: hi + lo rounds it to
-// within 2^-9 of its value (bf16: 2^-9), or 2^-21 of its block's largest.  Gate, up and silu stay in float32, the result is rounded
-// to bf16 once.
+// below that, half the lo part's smallest step of 2^-9 * 2^-4.  The activation
+// times its route's weight, operand of the second product, is stored the same way:
+// hi + lo rounds it to within 2^-9 of its value (bf16: 2^-9), or 2^-21 of its
+// block's largest.  Gate, up and silu stay in float32, the result is rounded to
+// bf16 once.
 //
 // Orientation as in experts.cu: 128 weight rows are the MMA's M side (four times
 // 16 gate rows and the 16 up rows of the same features, so that a feature's gate
-// and up meet in one warp; or 128 down rows), the routes its N side.  Groups are split into sub-groups of at most 32, 64 or 128 routes
-// (by the mean of the groups: small groups need no wide tiles, and narrow ones
-// leave shared memory to the weights), each with its own work items, so that a
-// popular expert is spread over the GPU.
+// and up meet in one warp; or 128 down rows), the routes its N side.  An item is
+// two such tiles, which share the routes, by a sub-group of up to 16, 48 or 112
+// routes (by the mean of the groups: few routes leave shared memory to the
+// weights; 112 is what two accumulators of two tiles leave room for beside the
+// scales).  A popular expert is many items, spread over the GPU.  One tile an
+// item, with two CTAs on an SM instead, loads the routes twice as often: 64 decode
+// tokens 44 us against 36, 4096 prompt tokens 429 against 342.
 //
-// Data flow of a step (128 columns): TMA unpacks the codes of 128 weight rows
-// into 16 KB of shared memory (4-bit data in 8-bit places, 128-byte swizzle, as
-// the MMA reads them) and brings the routes' hi and lo parts; cp.async brings
-// the weight rows' scale bytes, 4 a step, in pieces of 16, 8 or 4 as the rows are
-// aligned (no padding of the scale rows); four warps move the scales of both sides into tensor memory
-// (row r in lane r % 32 of every 32-lane quarter, column r / 32, one byte for
-// each 32 columns of the step); one thread issues the 8 MMAs of K = 32, hi and
-// lo for each scale byte.
+// Data flow of a step (128 columns): one TMA load unpacks the codes of 256 weight
+// rows into 32 KB of shared memory (4-bit data in 8-bit places, 128-byte swizzle, as
+// the MMA reads them), one brings the routes' hi and lo parts; the scale bytes of
+// four steps come in pieces of 16 bytes a row, by TMA or, where K is no multiple of
+// 512, by cp.async; two warps arrange them and tcgen05.cp copies them into tensor
+// memory (row r's bytes in lane r % 32 of every 32-lane quarter, column r / 32, a byte
+// for each 32 columns).  Up to 48 routes: hi and lo side by side in N, added up in the
+// epilogue, so that the weights are read once (four MMAs a tile); more: hi, then lo
+// into the same columns, the weights kept in the tensor core's buffer in between.
 //
-// CTA roles (352 threads): warp 0 claims work and loads codes; warp 1 issues the
-// MMAs; warps 2-5 drain the accumulators; warp 6 loads the routes; warps 9 and
-// 10 bring the weights' and the routes' scales, warps 7 and 8 arrange them.
-// Codes do not depend on phase 1, so warps 0 and 9 run ahead into phase 2 while
-// the routes' warps wait for the activations.  Two CTAs share an SM: what bounds
-// a CTA is the one thread behind each load or MMA (measured: a wait that is
-// already over 100 cycles, an expect 40, a TMA load 290, an MMA or scale copy
-// 45, a commit 85), and two have two of each.
+// CTA roles (512 threads): warp 0 claims work and loads codes; warps 1 and 2 issue a
+// tile's MMAs each; warps 3-10 drain the accumulators, four a tile; warp 11 loads the
+// routes; warps 12 and 13 arrange scales, warps 14 and 15 bring the weights' and the
+// routes'.  Codes do not depend on phase 1, so warps 0 and 14 run ahead into phase 2
+// while the routes' warps wait for the activations.
+//
+// What bounds it.  2048 x 768 experts, GPU time: 8 experts of one token 16 us, of
+// which the chain prepare - load - phase 1 - phase 2 without queueing is about 12
+// (32 experts of 256 x 128 take 12.1); 64 tokens (43 experts, 110 MB) 33.8 us: 8 before the
+// first load and after the last store, the rest at 4.9 TB/s, the first loads and the
+// wait for phase 1's last activations left out 5.6; 4096 tokens of 8 routes 320 us: 40 for
+// the routes' hi and lo parts (134 MB written), the rest at 1.0 PFLOP/s on the hi and
+// lo parts' products twice that, bounded by what comes from L2 into an SM (44 KB a
+// step, 33 bytes a cycle; 8 KB boxes that all lie in L2 reach 55) and by the power
+// limit (1.5 to 1.6 GHz while it runs).
+// Tried and left out: prefetching the next item into L2 (33.8 -> 38 to 40 us: the
+// loads of the item at hand wait behind it), routes gathered by cp.async in the
+// kernel (no prepared copies, but 36 -> 42 and 342 -> 335), 16 epilogue warps (34 ->
+// 39), four stages of 80 routes for three of 112 (321 -> 343), scales copied a step
+// ahead (321 -> 350).
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 

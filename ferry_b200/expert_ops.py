@@ -187,6 +187,10 @@ def route_experts(logits, topk, *, score='softmax', bias=None, n_group=1, topk_g
     softmax (a row of nothing else has weights 0); NaN scores are taken last
     and give NaN weights.  Scores are compared in 64 bits.  At most 1024
     experts, topk <= 32, n_group <= 32."""
+    done = _lib.fast().route_experts(logits, topk, score, bias, n_group, topk_group, group_score, norm_topk_prob,
+                                     scaling, weights_dtype)
+    if done is not None:
+        return done
     require_cuda(logits, bias)
     logits_type, weights_type = _lib.ELEMENT_TYPES.get(logits.dtype), _lib.ELEMENT_TYPES.get(weights_dtype)
     if logits_type is None or logits.dim() != 2:
@@ -261,6 +265,9 @@ def quantize_mxfp4(x, out=None):
     two codes a byte, the lower nibble first.  A block holding an infinity or
     a NaN has s = 255 and reads back as NaN.  `out`: (codes, scales) to write
     to, such as the two parts of expert rows (ferry_b200.model.mxfp4_parts)."""
+    done = _lib.fast().quantize_mxfp4(x) if out is None else None
+    if done is not None:
+        return done
     require_cuda(x)
     kind = _lib.ELEMENT_TYPES.get(x.dtype)
     if kind is None or x.dim() < 1:
@@ -284,6 +291,9 @@ def quantize_mxfp4(x, out=None):
 def dequantize_mxfp4(codes, scales, dtype=BF16, out=None):
     """The values of quantize_mxfp4's codes and scales, rounded once to `dtype`
     (bf16 and float32 hold them exactly, but for 6 * 2^127 and its like)."""
+    done = _lib.fast().dequantize_mxfp4(codes, scales, dtype) if out is None else None
+    if done is not None:
+        return done
     require_cuda(codes, scales, out)
     if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.dim() < 1:
         raise _lib.FerrybError('codes and scales must be uint8')
@@ -339,6 +349,10 @@ def execute_experts_mxfp4(cache, input, routing_weights, slots, starts, rows, co
     the call waits for the GPU and raises; with `err`, an int32 [1] CUDA tensor
     that starts at 0, it returns at once and leaves a non-zero code there for
     the caller to check, and can be captured into a CUDA graph."""
+    done = _lib.fast().execute_experts_mxfp4(cache, input, routing_weights, slots, starts, rows, cols, hidden,
+                                             intermediate, out, err)
+    if done is not None:
+        return done
     require_cuda(cache, input, routing_weights, slots, starts, rows, cols, out, err)
     dev, index = input.device, input.get_device()
     for t in (cache, routing_weights, slots, starts, rows, cols, out, err):

@@ -197,3 +197,18 @@ def test_row_parts():
     codes, scales = mxfp4_parts(rows)
     assert codes.shape == (2, 3 * 128 * 64 // 2) and scales.shape == (2, 3 * 128 * 64 // 32)
     assert codes.data_ptr() == rows.data_ptr() and int(scales[0, 0]) == codes.shape[1]
+
+
+def test_the_extension_leaves_what_is_not_plain():
+    """Built with the library; anything but plain CUDA tensors is left to the Python checks."""
+    fast = _lib.fast()
+    assert fast.__name__ == 'ferry_b200._fast'
+    x, v = torch.zeros(2, 32), torch.zeros(3, dtype=torch.int64)
+    assert fast.route_experts(x, 2, 'softmax', None, 1, 1, 'max', True, 1.0, BF16) is None
+    assert fast.quantize_mxfp4(x) is None and fast.dequantize_mxfp4(x, x, BF16) is None
+    assert fast.execute_experts_mxfp4(x, x, x, v, v, v, v, 128, 128, None, None) is None
+    for bad in (None, 7, 'x', [x]):
+        assert fast.quantize_mxfp4(bad) is None and fast.dequantize_mxfp4(bad, x, BF16) is None
+        assert fast.route_experts(bad, 2, 'softmax', None, 1, 1, 'max', True, 1.0, BF16) is None
+        assert fast.execute_experts_mxfp4(x, bad, x, v, v, v, v, 128, 128, None, None) is None
+    assert fast.route_experts() is None and fast.route_experts(x) is None
