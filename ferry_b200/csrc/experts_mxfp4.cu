@@ -372,6 +372,10 @@ __device__ __forceinline__ bool mx_wait_step(uint64_t* bars, uint32_t t, volatil
   return mx_wait(bars + t % kBars, (t / kBars) & 1, abort_flag, err);
 }
 
+// Count one up, after everything the warp wrote before its last __syncwarp.
+__device__ __forceinline__ void red_release_gpu(int* p) {
+  asm volatile("red.release.gpu.global.add.s32 [%0], 1;" ::"l"(p) : "memory");
+}
 // Wait until the sub-group's activations are written: four epilogue warps for
 // each of its phase-1 tiles.
 __device__ __forceinline__ bool mx_wait_dep(const int* dep, uint32_t want, volatile int* abort_flag,
@@ -888,9 +892,8 @@ __global__ void __launch_bounds__(kMxThreads, 1)
       if (++acc == 2) { acc = 0; acc_phase ^= 1; }
       if (it.phase == 1 && mine) {
         // publish this warp's activations to the sub-group's phase-2 items
-        __threadfence();
         __syncwarp();
-        if (lane == 0) atomicAdd(p.dep + it.group, 1);
+        if (lane == 0) red_release_gpu(p.dep + it.group);
       }
     }
   }
