@@ -224,6 +224,22 @@ def test_experts_match_definition(case):
     _assert_close(_run(d), d)
 
 
+@pytest.mark.parametrize('case', [
+    # enough groups that an item has two tiles of weight rows: narrow, middling and wide
+    # sub-groups, an odd number of down tiles, scale rows of 4, 8 and 16-byte multiples
+    ([1, 0, 3, 2] * 50, 128, 128, 5, 9, 4),
+    ([5, 17, 33, 0, 40] * 10, 384, 512, 6, 50, 4),
+    ([20, 60, 113] * 17, 384, 384, 4, 120, 8),
+    ([1, 250, 48, 49, 64] * 10, 512, 512, 3, 90, 6),
+    ([16] * 60, 640, 384, 2, 30, 3),
+], ids=lambda c: f'H{c[1]}_I{c[2]}_n{sum(c[0])}')
+def test_experts_of_many_groups(case):
+    d = _layer(*case)
+    got = _run(d)
+    _assert_close(got, d)
+    assert torch.equal(got, _run(d))
+
+
 def test_experts_weight_types_and_layout():
     from ferry_b200 import expert_ops
     d = _layer([9, 30, 2], 256, 256, 3, 20, 4)
