@@ -343,8 +343,11 @@ def execute_experts_mxfp4(cache, input, routing_weights, slots, starts, rows, co
     left as they were.  input is bf16, routing_weights [tokens, topk] bf16,
     fp16 or float32.  hidden and intermediate are multiples of 128.
 
-    Sums, gate and up are float32; the activation and the result are rounded
-    to bf16 once each.  Index errors are found on the device: the routes'
+    Sums, gate and up are float32, the result is rounded to bf16 once.  Inputs
+    and activations (times the route's weight) go into the products as two e4m3
+    numbers each, which hold a bf16 input down to 2^-13 of the largest of its 32
+    neighbours exactly and an activation to bf16's precision; a row that is not
+    finite comes out as NaN.  cache is 32-byte aligned.  Index errors are found on the device: the routes'
     rows become NaN (starts out of order: no row is written).  Without `err`
     the call waits for the GPU and raises; with `err`, an int32 [1] CUDA tensor
     that starts at 0, it returns at once and leaves a non-zero code there for

@@ -165,22 +165,28 @@ FERRYB_API int ferryb_dequantize_mxfp4(const void* codes, int64_t codes_stride, 
                                        int64_t scales_stride, int64_t rows, int64_t width, void* y,
                                        int32_t y_type, int64_t y_stride, ferryb_stream_t stream);
 
-/* Routed-expert SwiGLU over MXFP4 expert rows (tcgen05, weights expanded on
- * the way into tensor memory): ferryb_execute_experts for 4-bit experts, with
- * the group table on the device and no host synchronisation.
+/* Routed-expert SwiGLU over MXFP4 expert rows (tcgen05 with block-scaled
+ * operands: the 4-bit codes go into the products as they are):
+ * ferryb_execute_experts for 4-bit experts, with the group table on the device
+ * and no host synchronisation.
  *
- * cache: 16-byte aligned device bytes [cache_slots, 3 * hidden * intermediate
+ * cache: 32-byte aligned device bytes [cache_slots, 3 * hidden * intermediate
  * * 17 / 32]; a row is the codes of [gate I x H | up I x H | down H x I] (see
  * ferryb_quantize_mxfp4), then their scale bytes in the same order.  Group g
  * is routes [starts[g], starts[g + 1]) with the weights of slots[g]; groups may
  * be empty, and output rows of routes outside [starts[0], starts[n_groups])
  * are left as they were.  out[p] = (silu(x Wg^T) * (x Wu^T)) Wd^T *
- * routing_weights[rows[p], cols[p]], x = input[rows[p]], rounded to bf16 once;
- * the activation is rounded to bf16, gate and up are not.
+ * routing_weights[rows[p], cols[p]], x = input[rows[p]], rounded to bf16 once.
+ * The operands x and (silu(x Wg^T) * (x Wu^T)) * weight are held as the sum of
+ * two e4m3 numbers with a shared power of two for 32 of them: x exactly down to
+ * 2^-13 of the largest of its 32 and within 2^-21 of that below, the second
+ * within 2^-9 of its value (bf16's half step) or 2^-21 of the largest; gate and
+ * up are float32.  A row whose x or whose activation is not finite comes out as
+ * NaN.
  * Errors found on the device set *err (4, if it was 0) and go on: a row, column
  * or slot out of range makes its routes' outputs NaN; with starts out of order
- * or range no row is written.  *err = 1: a
- * wait inside the kernel ran out, no output is valid.
+ * or range no row is written.  *err = 1: a wait inside the kernel ran out, no
+ * output is valid.
  * hidden and intermediate: multiples of 128, at most 65536.  The workspace is
  * 256-byte aligned, not shared by calls that may overlap. */
 typedef struct ferryb_mxfp4_experts_args {
