@@ -100,6 +100,8 @@ constexpr uint32_t kTmemCols = 512, kTileCols = 112, kAccCols = kTiles * kTileCo
 constexpr uint32_t kMxSmem =
     kPoolBytes + kPlaces * (kTiles + 1) * kPieceBytes + kTilePool + kTiles * kXchgBytes + kBarBytes;
 static_assert(kMxSmem <= 227 * 1024, "shared memory");
+// one wrap at most when a block of steps is passed over in the ring of arranged scales
+static_assert(kTilePool / ((kTiles + 2) * 512) >= kBlock, "ring of arranged scales");
 constexpr uint64_t kMxWaitNs = 2000000000ull;  // bound on any wait
 
 // Up to 128 routes of one group.
