@@ -25,8 +25,8 @@
 // Orientation as in experts.cu: 128 weight rows are the MMA's M side (four times
 // 16 gate rows and the 16 up rows of the same features, so that a feature's gate
 // and up meet in one warp; or 128 down rows), the routes its N side.  An item is
-// two such tiles, which share the routes, by a sub-group of up to 16, 48 or 112
-// routes (by the mean of the groups: few routes leave shared memory to the
+// two such tiles, which share the routes, by a sub-group of up to 16, 32, 48, 64 or
+// 112 routes (by the mean of the groups: few routes leave shared memory to the
 // weights; 112 is what two accumulators of two tiles leave room for beside the
 // scales).  A popular expert is many items, spread over the GPU.  One tile an
 // item, with two CTAs on an SM instead, loads the routes twice as often: 64 decode
@@ -116,7 +116,7 @@ struct MxGroup {
 struct MxHeader {
   int queue;     // claim counter
   int n_groups;  // sub-groups
-  int cap;       // most routes of a sub-group: 16, 48 or 112
+  int cap;       // most routes of a sub-group: 16, 32, 48, 64 or 112
 };
 
 struct MxParams {
@@ -356,8 +356,8 @@ __device__ __forceinline__ bool mx_epilogue_all(int id, bool v) {
 // places of routes (hi and lo parts of `cap` rows), a step each.  More places
 // for codes where routes are few (memory-bound), as many of both where they
 // are many.
-__device__ __forceinline__ uint32_t mx_code_stages(int cap) { return cap <= 48 ? 5 : 3; }
-__device__ __forceinline__ uint32_t mx_route_stages(int cap) { return cap == 16 ? 4 : 3; }
+__device__ __forceinline__ uint32_t mx_code_stages(int cap) { return cap <= 48 ? 5 : cap == 64 ? 4 : 3; }
+__device__ __forceinline__ uint32_t mx_route_stages(int cap) { return cap <= 32 || cap == 64 ? 4 : 3; }
 
 // Rows of routes that a sub-group's tile holds: the next multiple of 16.
 __device__ __forceinline__ int mx_rows(int count) { return (count + 15) & ~15; }
@@ -963,10 +963,14 @@ __global__ void __launch_bounds__(kPrepThreads) mxfp4_prepare_kernel(const MxPre
     active = base;
     __syncthreads();
     if (threadIdx.x == 0) base = 0;
-    // sub-groups no wider than the mean group asks for
+    // sub-groups no wider than the mean group asks for: narrow ones leave shared memory
+    // to more loads under way, wide ones read the weights less often (128 experts of
+    // 2048 x 768, routes of a group in the mean: 16: 32 at most 36.2 us, 48 36.0, 112
+    // 40.2; 24: 50.2, 47.7, 53.2; 43: 72.9, 65.0, 65.9 and 64 63.4; 55: 87.2, 77.9, 74.1
+    // and 64 73.8)
     const int64_t all = a.starts[a.n_groups] - a.starts[0];
     const int64_t mean = active ? (all + active - 1) / active : 0;
-    const int cap = mean <= 4 ? 16 : mean <= 16 ? 48 : 112;
+    const int cap = mean <= 4 ? 16 : mean <= 16 ? 32 : mean <= 32 ? 48 : mean <= 56 ? 64 : 112;
     __syncthreads();
     // Sub-groups in descending order of their rows, so that the long epilogues of the
     // first product are over early and the work left at the end comes in small items:

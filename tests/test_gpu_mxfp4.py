@@ -232,6 +232,8 @@ def test_experts_match_definition(case):
     ([20, 60, 113] * 17, 384, 384, 4, 120, 8),
     ([1, 250, 48, 49, 64] * 10, 512, 512, 3, 90, 6),
     ([16] * 60, 640, 384, 2, 30, 3),
+    ([30, 12, 33, 49] * 10, 256, 512, 3, 40, 4),
+    ([64, 65, 20, 48, 1] * 10, 384, 512, 3, 70, 6),
 ], ids=lambda c: f'H{c[1]}_I{c[2]}_n{sum(c[0])}')
 def test_experts_of_many_groups(case):
     d = _layer(*case)
