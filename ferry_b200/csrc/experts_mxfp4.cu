@@ -940,6 +940,7 @@ constexpr int kPrepThreads = 256;
 __global__ void __launch_bounds__(kPrepThreads) mxfp4_prepare_kernel(const MxPrepare a) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   pdl_launch_dependents();  // the GEMM's CTAs may set up and wait
+  pdl_wait();
   if (blockIdx.x == 0) {
     __shared__ int warp_sum[kPrepThreads / 32];
     __shared__ int base;
@@ -1209,19 +1210,9 @@ static int launch_experts(const MxMaps& maps, const MxParams& p, const ferryb_mx
   }
   const int64_t subs = e->n_groups < e->routes ? e->n_groups + e->routes / 16 : e->routes;
   const int64_t items = subs * (p.mt1 + p.mt2), most = num_sms(device);
-  // programmatic dependent launch: the CTAs set up while the routes are prepared
-  cudaLaunchConfig_t lc{};
-  lc.gridDim = dim3(static_cast<unsigned>(items < most ? items : most));
-  lc.blockDim = dim3(kMxThreads);
-  lc.dynamicSmemBytes = kMxSmem;
-  lc.stream = stream;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  lc.attrs = &attr;
-  lc.numAttrs = 1;
-  FB_CUDA(cudaLaunchKernelEx(&lc, mxfp4_swiglu_kernel, maps, p));
-  return FERRYB_OK;
+  // the CTAs set up while the routes are prepared
+  return launch_behind(mxfp4_swiglu_kernel, static_cast<unsigned>(items < most ? items : most), kMxThreads, kMxSmem,
+                       stream, maps, p);
 }
 
 extern "C" int64_t ferryb_execute_experts_mxfp4_workspace(int64_t routes, int64_t n_groups,
@@ -1306,7 +1297,8 @@ extern "C" int ferryb_execute_experts_mxfp4(const ferryb_mxfp4_experts_args* e, 
 
   const int64_t gather = (e->routes + kPrepThreads / 32 - 1) / (kPrepThreads / 32);
   const int64_t most = 8 * static_cast<int64_t>(sms);
-  mxfp4_prepare_kernel<<<1 + static_cast<int>(gather < most ? gather : most), kPrepThreads, 0, stream>>>(pr);
-  FB_LAUNCH_CHECK();
+  if ((s = launch_behind(mxfp4_prepare_kernel, 1 + static_cast<unsigned>(gather < most ? gather : most),
+                         kPrepThreads, 0, stream, pr)))
+    return s;
   return launch_experts(maps, p, e, device, stream);
 }

@@ -70,6 +70,7 @@ template <typename T, int ALIGN>
 __global__ void __launch_bounds__(kMxThreads)
     quantize_mxfp4_kernel(const T* __restrict__ x, uint8_t* __restrict__ codes,
                           uint8_t* __restrict__ scales, const MxShape s) {
+  pdl_wait();
   const int64_t u0 = static_cast<int64_t>(blockIdx.x) * (kMxThreads * kMxUnroll) + threadIdx.x;
   float v[kMxUnroll][8];
   int64_t row[kMxUnroll], in_row[kMxUnroll];
@@ -152,6 +153,7 @@ template <typename T, int ALIGN>
 __global__ void __launch_bounds__(kMxThreads)
     dequantize_mxfp4_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                             T* __restrict__ y, const MxShape s) {
+  pdl_wait();
   const int64_t u0 = static_cast<int64_t>(blockIdx.x) * (kMxThreads * kMxUnroll) + threadIdx.x;
   uint32_t packed[kMxUnroll];
   int byte[kMxUnroll];
@@ -230,10 +232,8 @@ static int quantize_typed(const void* x, void* codes, void* scales, const MxShap
   const unsigned grid = static_cast<unsigned>((s.units + per - 1) / per);
   auto kernel = align == 0 ? quantize_mxfp4_kernel<T, 0> : quantize_mxfp4_kernel<T, 16>;
   if (sizeof(T) == 4 && align == 32) kernel = quantize_mxfp4_kernel<T, sizeof(T) == 4 ? 32 : 16>;
-  kernel<<<grid, kMxThreads, 0, stream>>>(static_cast<const T*>(x), static_cast<uint8_t*>(codes),
-                                          static_cast<uint8_t*>(scales), s);
-  FB_LAUNCH_CHECK();
-  return FERRYB_OK;
+  return launch_behind(kernel, grid, kMxThreads, 0, stream, static_cast<const T*>(x), static_cast<uint8_t*>(codes),
+                       static_cast<uint8_t*>(scales), s);
 }
 
 template <typename T>
@@ -243,10 +243,8 @@ static int dequantize_typed(const void* codes, const void* scales, void* y, cons
   const unsigned grid = static_cast<unsigned>((s.units + per - 1) / per);
   auto kernel = align == 0 ? dequantize_mxfp4_kernel<T, 0> : dequantize_mxfp4_kernel<T, 16>;
   if (sizeof(T) == 4 && align == 32) kernel = dequantize_mxfp4_kernel<T, sizeof(T) == 4 ? 32 : 16>;
-  kernel<<<grid, kMxThreads, 0, stream>>>(static_cast<const uint8_t*>(codes),
-                                          static_cast<const uint8_t*>(scales), static_cast<T*>(y), s);
-  FB_LAUNCH_CHECK();
-  return FERRYB_OK;
+  return launch_behind(kernel, grid, kMxThreads, 0, stream, static_cast<const uint8_t*>(codes),
+                       static_cast<const uint8_t*>(scales), static_cast<T*>(y), s);
 }
 
 }  // namespace ferryb

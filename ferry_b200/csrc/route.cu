@@ -325,6 +325,7 @@ __device__ __forceinline__ bool route_quick(const RouteArgs& a, int64_t t, int l
 
 template <typename T, int PER, bool SOFTMAX>
 __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RouteArgs a) {
+  pdl_wait();
   const int64_t t = static_cast<int64_t>(blockIdx.x) * kRouteWarps + (threadIdx.x >> 5);
   if (t >= a.tokens) return;
   const int lane = threadIdx.x & 31;
@@ -432,22 +433,20 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RouteArgs
 }
 
 template <typename T, int PER, bool SOFTMAX>
-static void route_launch(RouteArgs a, cudaStream_t stream) {
+static int route_launch(RouteArgs a, cudaStream_t stream) {
   const unsigned grid = static_cast<unsigned>((a.tokens + kRouteWarps - 1) / kRouteWarps);
   constexpr uintptr_t kVec = PER * sizeof(T) < 16 ? PER * sizeof(T) : 16;
   a.whole = a.per == PER && a.gsize == a.lpg * PER && reinterpret_cast<uintptr_t>(a.logits) % kVec == 0 &&
             (a.tokens <= 1 || a.row_stride * sizeof(T) % kVec == 0) &&
             reinterpret_cast<uintptr_t>(a.bias) % 16 == 0;
-  route_kernel<T, PER, SOFTMAX><<<grid, kRouteWarps * 32, 0, stream>>>(a);
+  return launch_behind(route_kernel<T, PER, SOFTMAX>, grid, kRouteWarps * 32, 0, stream, a);
 }
 template <typename T, bool SOFTMAX>
 static int route_per(const RouteArgs& a, cudaStream_t stream) {
-  if (a.per <= 4) route_launch<T, 4, SOFTMAX>(a, stream);
-  else if (a.per <= 8) route_launch<T, 8, SOFTMAX>(a, stream);
-  else if (a.per <= 16) route_launch<T, 16, SOFTMAX>(a, stream);
-  else route_launch<T, 32, SOFTMAX>(a, stream);
-  FB_LAUNCH_CHECK();
-  return FERRYB_OK;
+  if (a.per <= 4) return route_launch<T, 4, SOFTMAX>(a, stream);
+  if (a.per <= 8) return route_launch<T, 8, SOFTMAX>(a, stream);
+  if (a.per <= 16) return route_launch<T, 16, SOFTMAX>(a, stream);
+  return route_launch<T, 32, SOFTMAX>(a, stream);
 }
 
 template <typename T>
