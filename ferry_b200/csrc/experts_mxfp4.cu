@@ -48,20 +48,21 @@
 // routes'.  Codes do not depend on phase 1, so warps 0 and 14 run ahead into phase 2
 // while the routes' warps wait for the activations.
 //
-// What bounds it.  2048 x 768 experts, GPU time: 8 experts of one token 16 us, of
-// which the chain prepare - load - phase 1 - phase 2 without queueing is about 12
-// (32 experts of 256 x 128 take 12.1); 64 tokens (43 experts, 110 MB) 33.8 us: 8 before the
-// first load and after the last store, the rest at 4.9 TB/s, the first loads and the
-// wait for phase 1's last activations left out 5.6; 4096 tokens of 8 routes 320 us: 40 for
-// the routes' hi and lo parts (134 MB written), the rest at 1.0 PFLOP/s on the hi and
-// lo parts' products twice that, bounded by what comes from L2 into an SM (44 KB a
-// step, 33 bytes a cycle; 8 KB boxes that all lie in L2 reach 55) and by the power
-// limit (1.5 to 1.6 GHz while it runs).
-// Tried and left out: prefetching the next item into L2 (33.8 -> 38 to 40 us: the
-// loads of the item at hand wait behind it), routes gathered by cp.async in the
-// kernel (no prepared copies, but 36 -> 42 and 342 -> 335), 16 epilogue warps (34 ->
-// 39), four stages of 80 routes for three of 112 (321 -> 343), scales copied a step
-// ahead (321 -> 350).
+// What bounds it.  2048 x 768 experts, GPU time: 8 experts of one token 16.4 us, of
+// which the chain prepare - claim - load - phase 1 - phase 2 without queueing is about
+// 11 (32 experts of 256 x 128 take 11.5); 64 tokens (43 experts, 110 MB) 32.5 us: 8
+// before the first load and after the last store, phase 1 at 5.6 TB/s, about 5 lost in
+// the change of phase and with the last items; 4096 tokens of 8 routes 315 us (375 when
+// it runs on and the power limit brings the clock to 1.5 GHz): 40 for the routes' hi and
+// lo parts (134 MB written), then 1,220 cycles a step whose MMAs take 750: loads are
+// under way for 1,900 cycles (850 alone), 33 bytes a cycle into the SM where tiles that
+// all lie in a corner of L2 come at 40 to 55.  Half the route bytes, or half the MMAs,
+// change a step by 3 to 6 %.
+// Tried and left out: prefetching the next item into L2 (64 tokens 34 -> 38 to 40 us:
+// the loads of the item at hand wait behind it), routes gathered by cp.async in the
+// kernel (no prepared copies, but 36 -> 42, and 342 -> 335), 16 epilogue warps (34 ->
+// 39), scales copied a step ahead (321 -> 350), four stages of 80 routes for three of
+// 112 (321 -> 343), one tile an item where groups are few (8 experts 16.1 -> 17.2).
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
@@ -169,7 +170,7 @@ __device__ __forceinline__ MxItem mx_item(const MxParams& p, int n_groups, int i
 }
 
 // One wait of at most about 20 us: the hint lets the hardware suspend the warp,
-// which otherwise polls and takes issue slots from the warps that expand.
+// which otherwise polls and takes issue slots from the warps that work.
 __device__ __forceinline__ bool mx_try_wait(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
