@@ -940,8 +940,10 @@ constexpr int kPrepThreads = 256;
 
 __global__ void __launch_bounds__(kPrepThreads) mxfp4_prepare_kernel(const MxPrepare a) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  pdl_launch_dependents();  // the GEMM's CTAs may set up and wait
+  // First wait for what the stream ran before, then let the GEMM's CTAs set up and wait:
+  // they fill the SMs, and must not while an earlier kernel may need another stream's.
   pdl_wait();
+  pdl_launch_dependents();
   if (blockIdx.x == 0) {
     __shared__ int warp_sum[kPrepThreads / 32];
     __shared__ int base;

@@ -117,3 +117,56 @@ def test_streams_and_graphs(taken):
     x.mul_(3)
     g.replay()
     assert torch.equal(back, expert_ops.dequantize_mxfp4(*expert_ops.quantize_mxfp4(x), torch.float32))
+
+
+def test_offsets_beyond_32_bits(taken):
+    """Rows further than 2^32 elements apart, and a cache slot that starts beyond 4 GiB."""
+    from ferry_b200 import expert_ops
+    from ferry_b200.model import mxfp4_row_bytes
+    far = 2 ** 32 + 64
+    x = torch.empty(far + 64, dtype=BF16, device=DEV).as_strided((2, 64), (far, 1))
+    x.copy_(torch.randn(2, 64))
+    near = x.contiguous()
+    for got, want in zip(expert_ops.route_experts(x, 4), expert_ops.route_experts(near, 4)):
+        assert torch.equal(got, want)
+    codes, scales = expert_ops.quantize_mxfp4(x)
+    assert taken['route_experts'] and taken['quantize_mxfp4']
+    for got, want in zip((codes, scales), expert_ops.quantize_mxfp4(near)):
+        assert torch.equal(got, want)
+    expert_ops.dequantize_mxfp4(codes, scales, BF16, out=x)
+    assert torch.equal(x, expert_ops.dequantize_mxfp4(codes, scales))
+    del x
+    H, I = 2048, 1408
+    size = mxfp4_row_bytes(H, I)
+    slots = 2 ** 32 // size + 3
+    cache = torch.empty(slots, size, dtype=torch.uint8, device=DEV)
+    g = torch.Generator(device=DEV).manual_seed(0)
+    cache[0] = torch.randint(0, 256, (size,), generator=g, dtype=torch.uint8, device=DEV)
+    cache[0, 3 * H * I // 2:] = 117
+    cache[-1] = cache[0]
+    y = torch.randn(3, H, device=DEV).to(BF16)
+    w = torch.rand(3, 1, device=DEV)
+    rows, cols = torch.arange(3, device=DEV), torch.zeros(3, dtype=torch.int64, device=DEV)
+    starts, err = torch.tensor([0, 3], device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    a, b = (expert_ops.execute_experts_mxfp4(cache, y, w, torch.tensor([s], device=DEV), starts, rows, cols, H, I,
+                                             err=err) for s in (0, slots - 1))
+    assert int(err) == 0 and torch.equal(a, b) and bool((a != 0).any())
+
+
+def test_back_to_back_calls_see_each_other():
+    """A chain in which each launch reads what the one before it wrote, far longer
+    than the launch queue's overlap."""
+    from ferry_b200 import expert_ops
+    x = torch.randn(64, 4096, device=DEV)
+    want = expert_ops.dequantize_mxfp4(*expert_ops.quantize_mxfp4(x), torch.float32)
+    y = x
+    for _ in range(50):
+        y = expert_ops.dequantize_mxfp4(*expert_ops.quantize_mxfp4(y), torch.float32)  # quantised values stay
+    assert torch.equal(y, want)
+    for _ in range(50):
+        y = y * -1                        # a kernel of torch between
+        c, s = expert_ops.quantize_mxfp4(y)
+        y = expert_ops.dequantize_mxfp4(c, s, torch.float32)
+        sel, w = expert_ops.route_experts(y[:, :128], 2)
+    assert torch.equal(y, want)
+    assert torch.equal(sel, expert_ops.route_experts(want[:, :128].contiguous(), 2)[0])
