@@ -48,12 +48,12 @@
 // routes'.  Codes do not depend on phase 1, so warps 0 and 14 run ahead into phase 2
 // while the routes' warps wait for the activations.
 //
-// What bounds it.  2048 x 768 experts, GPU time: 8 experts of one token 16.4 us, of
+// What bounds it.  2048 x 768 experts, GPU time: 8 experts of one token 15.6 us, of
 // which the chain prepare - claim - load - phase 1 - phase 2 without queueing is about
 // 11 (32 experts of 256 x 128 take 11.5); 64 tokens (43 experts, 110 MB) 32.5 us: 8
 // before the first load and after the last store, phase 1 at 5.6 TB/s, about 5 lost in
-// the change of phase and with the last items; 4096 tokens of 8 routes 315 us (375 when
-// it runs on and the power limit brings the clock to 1.5 GHz): 40 for the routes' hi and
+// the change of phase and with the last items; 4096 tokens of 8 routes 310 us (371 when
+// it runs on and the power limit brings the clock to 1.5 GHz): 36 for the routes' hi and
 // lo parts (134 MB written), then 1,220 cycles a step whose MMAs take 750: loads are
 // under way for 1,900 cycles (850 alone), 33 bytes a cycle into the SM where tiles that
 // all lie in a corner of L2 come at 40 to 55.  Half the route bytes, or half the MMAs,
