@@ -242,6 +242,50 @@ def test_experts_of_many_groups(case):
     assert torch.equal(got, _run(d))
 
 
+@pytest.mark.parametrize('case', [
+    # more groups than a block of the table's kernel has threads, with and without an
+    # order by size; the widest rows either way; one group of many sub-groups
+    ([1, 0, 20, 2, 0, 33] * 70, 128, 128, 3, 9, 4),
+    ([0] * 300 + [2, 0, 1], 128, 256, 2, 5, 2),
+    ([3], 65536, 128, 1, 3, 2),
+    ([2, 1], 128, 65536, 2, 3, 2),
+    ([4001], 128, 128, 1, 500, 8),
+], ids=lambda c: f'G{len(c[0])}_H{c[1]}_I{c[2]}')
+def test_experts_at_the_edges(case):
+    d = _layer(*case)
+    _assert_close(_run(d), d)
+
+
+def test_bad_slots_among_many_groups():
+    d = _layer([1, 0, 20, 2, 0, 33] * 70, 128, 128, 3, 9, 4)
+    good = _run(d)
+    slots = d['slots'].clone()
+    slots[[2, 3, 417]] = torch.tensor([3, -1, 2 ** 40])
+    slots[1] = 77  # of an empty group: not looked at
+    err = torch.zeros(1, dtype=torch.int32, device=DEV)
+    got = _run(dict(d, slots=slots), err=err)
+    bad = torch.zeros(len(d['rows']), dtype=torch.bool)
+    for g in (2, 3):
+        bad[d['starts'][g]:d['starts'][g + 1]] = True
+    bad[d['starts'][417]:d['starts'][418]] = True
+    assert int(err) == 4 and bool(got[bad.to(DEV)].isnan().all())
+    assert torch.equal(got[~bad.to(DEV)], good[~bad.to(DEV)])
+
+
+def test_output_over_the_input():
+    """out may be the rows that input was: they are read before any is written."""
+    d = _layer([5, 60, 3], 256, 128, 3, 68, 1)
+    d['rows'] = torch.randperm(68, generator=torch.Generator().manual_seed(1))
+    d['cols'] = torch.zeros(68, dtype=torch.int64)
+    want = _run(d)
+    t = {k: d[k].to(DEV) for k in ('cache', 'x', 'w', 'slots', 'starts', 'rows', 'cols')}
+    from ferry_b200 import expert_ops
+    err = torch.zeros(1, dtype=torch.int32, device=DEV)
+    got = expert_ops.execute_experts_mxfp4(t['cache'], t['x'], t['w'], t['slots'], t['starts'], t['rows'], t['cols'],
+                                           256, 128, out=t['x'], err=err)
+    assert got.data_ptr() == t['x'].data_ptr() and torch.equal(got, want) and int(err) == 0
+
+
 def test_experts_weight_types_and_layout():
     from ferry_b200 import expert_ops
     d = _layer([9, 30, 2], 256, 256, 3, 20, 4)
