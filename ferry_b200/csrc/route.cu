@@ -144,6 +144,10 @@ __device__ __forceinline__ void store_weight(const RouteArgs& a, int64_t at, dou
 // ordered if they lie 2 (75 + 3.4 x) k apart; without x, 2 (75 + 3.4 * 88) k.
 // Sigmoid: (1 - s) (4 + 2.4 |l|) from exp(-l), 5 for sum and quotient; that is s (4 +
 // 2.4 * 88 + 5) at most, and 7 against a score of 1.
+// A group's worth is off by the errors of its one or two keys: without a bias the share
+// of them at x = 88 (374, 220), with one twice 75 or 7 of the largest score, and the
+// roundings of each key's and their sum's addition, at most twice the keys' magnitudes.
+// Scores below e^-88, which leave float's range, cannot be selected here (kFar).
 // The key sort below drops the lowest bits of a key: 2^kBits of its units.
 constexpr float kUnit = 1.0f / (1 << 24);
 constexpr float kFar = 80.0f;  // scores further than e^-80 from the largest are left to 64 bits
@@ -223,7 +227,8 @@ __device__ __forceinline__ bool route_quick(const RouteArgs& a, int64_t t, int l
       second = fmaxf(fminf(best, ob), fmaxf(second, os));
       best = fmaxf(best, ob);
     }
-    const uint32_t worth = order_of(a.top2 ? best + second : best);
+    const float sum = a.top2 ? best + second : best;
+    const uint32_t worth = order_of(sum);
     int rank = 0;
     for (int g = 0; g < a.groups; ++g) {
       const uint32_t w = __shfl_sync(kAll, worth, g * a.lpg);
@@ -232,9 +237,16 @@ __device__ __forceinline__ bool route_quick(const RouteArgs& a, int64_t t, int l
     const bool stays = rank < a.kept;
     if (a.kept < a.groups) {
       const bool real = group < a.groups;
-      const float in = from_order(__reduce_min_sync(kAll, real && stays ? worth : 0xffffffffu));
-      const float out = from_order(__reduce_max_sync(kAll, real && !stays ? worth : 0u));
-      if (!(in - out > 2.0f * gap(in, 88.0f))) return false;  // a sum of two has both errors
+      // How far this worth may be off: as far as the keys in it, each of which was rounded
+      // at its own size (a sum of 1000.4 and -999.6 is off by the steps of 1000), and the
+      // rounding of their sum.  The groups are certain if the least that a kept one may be
+      // worth is above the most that a dropped one may be.
+      const float keys = fabsf(best) + (a.top2 ? fabsf(second) : 0.0f);
+      const float off = a.bias ? kUnit * ((SOFTMAX ? 160.0f : 16.0f) * largest + 4.0f * keys)
+                               : kUnit * (SOFTMAX ? 384.0f : 256.0f) * keys;
+      const float in = from_order(__reduce_min_sync(kAll, real && stays ? order_of(sum - off) : 0xffffffffu));
+      const float out = from_order(__reduce_max_sync(kAll, real && !stays ? order_of(sum + off) : 0u));
+      if (!(in > out)) return false;
     }
     if (!stays) mine = 0;
   }

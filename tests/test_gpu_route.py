@@ -185,3 +185,38 @@ def test_ties_across_the_border():
         for topk in (1, 8, 17, 32):
             _check(x, topk, score=score)
             _check(x, topk, score=score, bias=torch.arange(128).remainder(3).float() * 0.25)
+
+
+def _close_worths(tokens, size, seed):
+    """Logits of four experts in two groups, and biases (size, -size) in each, such
+    that the two groups' sums of keys lie a few float32 steps of `size` apart, for
+    softmax scores (the logits are log s with sum s = 1) and for sigmoid scores."""
+    g = np.random.default_rng(seed)
+    s = g.uniform(0.2, 0.8, (tokens, 4))
+    apart = g.uniform(-1, 1, tokens) * np.minimum(4 * size * 2.0 ** -24, 0.1)
+    soft = s.copy()
+    soft[:, 2:] *= ((soft[:, :2].sum(1) + apart) / soft[:, 2:].sum(1))[:, None]
+    s[:, 3] = np.clip(s[:, 0] + s[:, 1] - s[:, 2] + apart, 0.01, 0.99)
+    bias = torch.tensor([size, -size, size, -size], dtype=torch.float32)
+    return {'softmax': torch.from_numpy(np.log(soft)).float(),
+            'sigmoid': torch.from_numpy(np.log(s / (1 - s))).float()}, bias
+
+
+@pytest.mark.parametrize('score', ['softmax', 'sigmoid'])
+@pytest.mark.parametrize('size', [1.0, 64.0, 256.0, 1e4, 1e6])
+def test_group_sums_of_biases_that_cancel(size, score):
+    """The two largest keys of a group may be far larger than their sum, and are
+    rounded at their own size."""
+    logits, bias = _close_worths(600, size, int(size))
+    kw = dict(score=score, n_group=2, topk_group=1, group_score='top2')
+    _check(logits[score], 2, bias=bias, **kw)
+    wide = torch.cat((logits[score], _logits(600, 28, 1)), 1)  # of 16 groups, 5 stay
+    _check(wide, 6, bias=torch.cat((bias, torch.zeros(28))), score=score, n_group=16, topk_group=5, group_score='top2')
+
+
+def test_group_sums_that_float32_orders_the_other_way():
+    """Worths of 0.7950212 and 0.7950132; float32 has 0.7949829 and 0.7950440."""
+    x = torch.tensor([[-0.33179307, -0.50137854, -1.0042144, 0.10770209]])
+    sel, _ = _check(x, 2, bias=torch.tensor([1000.0, -1000.0, 1000.0, -1000.0]), score='sigmoid', n_group=2,
+                    topk_group=1, group_score='top2')
+    assert sel.tolist() == [[0, 1]]
