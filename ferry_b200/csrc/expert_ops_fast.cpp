@@ -224,7 +224,8 @@ PyObject* experts(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (a[9] != Py_None) {
     given = cuda_tensor(a[9], device);
     if (!given || given->scalar_type() != at::kBFloat16 || given->dim() != 2 || given->size(0) != e.routes ||
-        given->size(1) != e.hidden || !given->is_contiguous())
+        given->size(1) != e.hidden || !given->is_contiguous() ||
+        reinterpret_cast<uintptr_t>(given->const_data_ptr()) % 4)
       Py_RETURN_NONE;
   }
   e.workspace_bytes = workspace_fn(e.routes, e.n_groups, e.hidden, e.intermediate);

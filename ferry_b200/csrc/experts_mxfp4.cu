@@ -1254,6 +1254,14 @@ extern "C" int ferryb_execute_experts_mxfp4(const ferryb_mxfp4_experts_args* e, 
                    reinterpret_cast<uintptr_t>(e->input) % 16 == 0 &&
                    (e->n_input <= 1 || (e->input_stride % 8 == 0 && e->input_stride >= e->hidden)),
                "execute_experts_mxfp4: the cache must be 32-byte, input rows 16-byte aligned");
+  // the epilogue stores pairs of bf16
+  FB_CHECK_ARG(reinterpret_cast<uintptr_t>(e->out) % 4 == 0, "execute_experts_mxfp4: out must be 4-byte aligned");
+  FB_CHECK_ARG((reinterpret_cast<uintptr_t>(e->slots) | reinterpret_cast<uintptr_t>(e->starts) |
+                reinterpret_cast<uintptr_t>(e->rows) | reinterpret_cast<uintptr_t>(e->cols)) % 8 == 0 &&
+                   reinterpret_cast<uintptr_t>(e->err) % 4 == 0 &&
+                   reinterpret_cast<uintptr_t>(e->routing_weights) % (e->weights_type == FERRYB_FP32 ? 4 : 2) == 0,
+               "execute_experts_mxfp4: slots, starts, rows, cols, err and routing_weights must be aligned to "
+               "their elements");
   const MxWs ws = mx_ws(e->routes, e->n_groups, e->hidden, e->intermediate);
   FB_CHECK_ARG(e->workspace && reinterpret_cast<uintptr_t>(e->workspace) % 256 == 0 &&
                    e->workspace_bytes >= ws.total,

@@ -347,11 +347,13 @@ def execute_experts_mxfp4(cache, input, routing_weights, slots, starts, rows, co
     and activations (times the route's weight) go into the products as two e4m3
     numbers each, which hold a bf16 input down to 2^-13 of the largest of its 32
     neighbours exactly and an activation to bf16's precision; a row that is not
-    finite comes out as NaN.  cache is 32-byte aligned.  Index errors are found on the device: the routes'
-    rows become NaN (starts out of order: no row is written).  Without `err`
-    the call waits for the GPU and raises; with `err`, an int32 [1] CUDA tensor
-    that starts at 0, it returns at once and leaves a non-zero code there for
-    the caller to check, and can be captured into a CUDA graph."""
+    finite comes out as NaN.  cache is 32-byte aligned, `out` 4-byte aligned (a
+    contiguous bf16 view that starts at an odd element is refused).  Index errors
+    are found on the device: the routes' rows become NaN (starts out of order: no
+    row is written).  Without `err` the call waits for the GPU and raises; with
+    `err`, an int32 [1] CUDA tensor that starts at 0, it returns at once and
+    leaves a non-zero code there for the caller to check, and can be captured
+    into a CUDA graph."""
     done = _lib.fast().execute_experts_mxfp4(cache, input, routing_weights, slots, starts, rows, cols, hidden,
                                              intermediate, out, err)
     if done is not None:
@@ -386,6 +388,8 @@ def execute_experts_mxfp4(cache, input, routing_weights, slots, starts, rows, co
         out = input.new_empty((routes, hidden))
     elif out.dtype != BF16 or out.shape != (routes, hidden) or not out.is_contiguous():
         raise _lib.FerrybError(f'out must be contiguous bf16 [{routes}, {hidden}]')
+    elif out.data_ptr() % 4:
+        raise _lib.FerrybError('out must be 4-byte aligned')
     wait = err is None
     if not wait:
         _check(err.dtype == torch.int32 and err.numel() == 1, 'err must be an int32 tensor of one element')

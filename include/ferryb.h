@@ -203,7 +203,7 @@ typedef struct ferryb_mxfp4_experts_args {
   const int64_t* rows;         /* device [routes] */
   const int64_t* cols;         /* device [routes] */
   int64_t routes, hidden, intermediate;
-  void* out;                   /* device bf16 [routes, hidden] */
+  void* out;                   /* device bf16 [routes, hidden], 4-byte aligned */
   void* workspace;
   int64_t workspace_bytes;
   int32_t* err;                /* device [1] */

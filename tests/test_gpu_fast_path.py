@@ -170,3 +170,23 @@ def test_back_to_back_calls_see_each_other():
         sel, w = expert_ops.route_experts(y[:, :128], 2)
     assert torch.equal(y, want)
     assert torch.equal(sel, expert_ops.route_experts(want[:, :128].contiguous(), 2)[0])
+
+
+def test_output_at_an_odd_element_is_refused(taken):
+    """Before anything is launched, by the short way too."""
+    from ferry_b200 import expert_ops
+    from ferry_b200.model import mxfp4_row_bytes
+    H, I = 128, 128
+    cache = torch.full((1, mxfp4_row_bytes(H, I)), 118, dtype=torch.uint8, device=DEV)
+    x, w = torch.randn(3, H, device=DEV).to(BF16), torch.rand(3, 1, device=DEV)
+    ids = lambda *v: torch.tensor(v, device=DEV)
+    args = (cache, x, w, ids(0), ids(0, 3), ids(0, 1, 2), ids(0, 0, 0), H, I)
+    err = torch.zeros(1, dtype=torch.int32, device=DEV)
+    buf = torch.full((3 * H + 4,), 7.0, dtype=BF16, device=DEV)
+    for kw in (dict(), dict(err=err)):
+        with pytest.raises(RuntimeError, match='4-byte aligned'):
+            expert_ops.execute_experts_mxfp4(*args, out=buf[1:1 + 3 * H].view(3, H), **kw)
+        assert not taken['execute_experts_mxfp4'] and bool((buf == 7).all())
+    got = expert_ops.execute_experts_mxfp4(*args, out=buf[2:2 + 3 * H].view(3, H), err=err)
+    assert taken['execute_experts_mxfp4'] and torch.equal(got, expert_ops.execute_experts_mxfp4(*args))
+    assert bool((buf[:2] == 7).all()) and bool((buf[2 + 3 * H:] == 7).all()) and int(err) == 0

@@ -212,3 +212,28 @@ def test_the_extension_leaves_what_is_not_plain():
         assert fast.route_experts(bad, 2, 'softmax', None, 1, 1, 'max', True, 1.0, BF16) is None
         assert fast.execute_experts_mxfp4(x, bad, x, v, v, v, v, 128, 128, None, None) is None
     assert fast.route_experts() is None and fast.route_experts(x) is None
+
+
+def test_experts_output_at_an_odd_element_is_refused(calls):
+    """The kernel stores bf16 pairs; contiguous views may start at any element."""
+    a = _experts_args()
+    buf = torch.zeros(9 * 128 + 2, dtype=BF16)
+    with pytest.raises(FerrybError, match='4-byte aligned'):
+        expert_ops.execute_experts_mxfp4(**dict(a, out=buf[1:-1].view(9, 128)))
+    assert not calls
+    expert_ops.execute_experts_mxfp4(**dict(a, out=buf[2:].view(9, 128)))
+    assert len(calls) == 1
+
+
+@pytest.mark.parametrize('change', [dict(out=0x1002), dict(out=0x1001), dict(err=0x1002), dict(slots=0x1004),
+                                    dict(starts=0x1004), dict(rows=0x1004), dict(cols=0x1004),
+                                    dict(routing_weights=0x1002)], ids=str)
+def test_experts_entry_refuses_misaligned_pointers(change):
+    lib = _lib.lib()
+    ws = lib.ferryb_execute_experts_mxfp4_workspace(9, 3, 128, 256)
+    a = _lib.Mxfp4ExpertsArgs(0x1000, 2, 0x1000, 6, 128, 0x1000, 2, 2, 0, 0x1000, 0x1000, 3, 0x1000, 0x1000, 9, 128,
+                              256, 0x1000, 0x1000, ws, 0x1000)
+    for k, v in change.items():
+        setattr(a, k, v)
+    assert lib.ferryb_execute_experts_mxfp4(ctypes.byref(a), None) == 1
+    assert b'aligned' in lib.ferryb_last_error()
