@@ -22,6 +22,9 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cfloat>
+#include <cmath>
+
 #include "ferryb.h"
 
 namespace {
@@ -90,6 +93,8 @@ PyObject* route(PyObject*, PyObject* const* a, Py_ssize_t n) {
       !to_int(a[5], 1, 32, &topk_group) || !PyBool_Check(a[7]) || !PyFloat_CheckExact(a[8]) ||
       !THPDtype_Check(a[9]))
     Py_RETURN_NONE;
+  const double scaling = PyFloat_AS_DOUBLE(a[8]);
+  if (std::isfinite(scaling) && std::fabs(scaling) > FLT_MAX) Py_RETURN_NONE;  // refused if it rounds to infinity
   r.tokens = logits.size(0);
   r.experts = static_cast<int32_t>(logits.size(1) > 1024 ? 1025 : logits.size(1));
   r.row_stride = logits.stride(0);
@@ -114,7 +119,7 @@ PyObject* route(PyObject*, PyObject* const* a, Py_ssize_t n) {
   r.n_group = static_cast<int32_t>(n_group);
   r.topk_group = static_cast<int32_t>(topk_group);
   r.norm_topk = a[7] == Py_True;
-  r.scaling = static_cast<float>(PyFloat_AS_DOUBLE(a[8]));
+  r.scaling = static_cast<float>(scaling);
   r.selected = selected.mutable_data_ptr<int64_t>();
   r.weights = weights.mutable_data_ptr();
   if (route_fn(&r, stream_of(device))) Py_RETURN_NONE;

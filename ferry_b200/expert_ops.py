@@ -14,6 +14,7 @@ captured into a CUDA graph.
 """
 import ctypes
 import functools
+import math
 import struct
 
 import torch
@@ -211,16 +212,18 @@ def route_experts(logits, topk, *, score='softmax', bias=None, n_group=1, topk_g
     topk = int(topk)
     if not 0 < topk <= experts:
         raise _lib.FerrybError(f'topk must be in [1, {experts}]')
+    scaling = float(scaling)
+    if math.isinf(ctypes.c_float(scaling).value) and not math.isinf(scaling):
+        raise _lib.FerrybError(f'scaling ({scaling}) is beyond float32')
     selected = logits.new_empty((tokens, topk), dtype=torch.int64)
     weights = logits.new_empty((tokens, topk), dtype=weights_dtype)
     try:
         args = _lib.pack_route_args(
             logits.data_ptr(), tokens, logits.stride(0), experts, topk, int(n_group), int(topk_group), logits_type,
-            weights_type, SCORES[score], GROUP_SCORES[group_score], int(bool(norm_topk_prob)), float(scaling),
+            weights_type, SCORES[score], GROUP_SCORES[group_score], int(bool(norm_topk_prob)), scaling,
             _lib.addr(bias), selected.data_ptr(), weights.data_ptr())
     except (struct.error, OverflowError):
-        raise _lib.FerrybError(f'n_group ({n_group}), topk_group ({topk_group}) or scaling ({scaling}) is too '
-                               'large') from None
+        raise _lib.FerrybError(f'n_group ({n_group}) or topk_group ({topk_group}) is too large') from None
     _cuda_call(dev, 'ferryb_route_experts', args)
     return selected, weights
 

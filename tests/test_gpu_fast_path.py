@@ -190,3 +190,21 @@ def test_output_at_an_odd_element_is_refused(taken):
     got = expert_ops.execute_experts_mxfp4(*args, out=buf[2:2 + 3 * H].view(3, H), err=err)
     assert taken['execute_experts_mxfp4'] and torch.equal(got, expert_ops.execute_experts_mxfp4(*args))
     assert bool((buf[:2] == 7).all()) and bool((buf[2 + 3 * H:] == 7).all()) and int(err) == 0
+
+
+@pytest.mark.parametrize('scaling', [1e39, -1e39, 3.4028235677973366e38, 1.7e308])
+def test_scaling_beyond_float32_is_refused_by_both_ways(taken, scaling):
+    from ferry_b200 import expert_ops
+    x = torch.randn(3, 16, device=DEV)
+    with pytest.raises(RuntimeError, match='scaling'):
+        expert_ops.route_experts(x, 2, scaling=scaling)
+    assert not taken['route_experts']
+
+
+@pytest.mark.parametrize('scaling', [3.4028234663852886e38, -3.4028235e38, float('inf'), float('nan'), 0.0, 1e-46])
+def test_scaling_at_the_ends_of_float32(taken, monkeypatch, scaling):
+    from ferry_b200 import expert_ops
+    x = torch.randn(3, 16, device=DEV)
+    (a, v), (b, w) = _both(monkeypatch, lambda: expert_ops.route_experts(x, 2, scaling=scaling,
+                                                                         weights_dtype=torch.float32))
+    assert torch.equal(a, b) and torch.equal(v.nan_to_num(7.0), w.nan_to_num(7.0))

@@ -237,3 +237,13 @@ def test_experts_entry_refuses_misaligned_pointers(change):
         setattr(a, k, v)
     assert lib.ferryb_execute_experts_mxfp4(ctypes.byref(a), None) == 1
     assert b'aligned' in lib.ferryb_last_error()
+
+
+@pytest.mark.parametrize('scaling', [1e39, -1e39, 3.4028235677973366e38, 1.7e308])
+def test_route_refuses_a_scaling_beyond_float32(calls, scaling):
+    with pytest.raises(FerrybError, match='scaling'):
+        expert_ops.route_experts(torch.zeros(3, 8), 2, scaling=scaling)
+    assert not calls
+    expert_ops.route_experts(torch.zeros(3, 8), 2, scaling=float('inf'))
+    expert_ops.route_experts(torch.zeros(3, 8), 2, scaling=-3.4028234663852886e38)
+    assert len(calls) == 2
