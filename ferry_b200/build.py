@@ -1,4 +1,5 @@
-"""Build libferryb.so (sm_100a) and _fast.so in-tree: python -m ferry_b200.build"""
+"""Build libferryb.so (sm_100a) and, where this interpreter's torch allows it, _fast.so
+in-tree: python -m ferry_b200.build"""
 import os
 import subprocess
 import sys
@@ -12,6 +13,8 @@ def build(jobs=None, verbose=False):
     out = subprocess.run(['make', '-C', str(CSRC), f'-j{jobs}', f'PYTHON={sys.executable}'], capture_output=not verbose, text=True)
     if out.returncode != 0:
         raise RuntimeError('libferryb build failed:\n' + (out.stdout or '') + (out.stderr or ''))
+    if not verbose and not (CSRC.parent / '_fast.so').exists():  # make has said why
+        print((out.stderr or '') + out.stdout[-1000:], file=sys.stderr)
     return CSRC.parent / 'libferryb.so'
 
 
