@@ -7,6 +7,8 @@ as the reference's TORCH_CHECKs raise RuntimeError into Python
 """
 import ctypes
 import struct
+import sys
+import warnings
 from pathlib import Path
 
 import torch
@@ -203,6 +205,12 @@ class _NoFast:
     route_experts = quantize_mxfp4 = dequantize_mxfp4 = execute_experts_mxfp4 = _none
 
 
+def _fast_is_of_this_process(module):
+    """An extension sees torch's C++ objects as its own torch had them."""
+    built = getattr(module, 'torch_version', None), getattr(module, 'python_version', '').split('.')[:2]
+    return built == (str(torch.__version__), [str(n) for n in sys.version_info[:2]])
+
+
 def fast():
     """The _fast extension (csrc/expert_ops_fast.cpp), which answers the plain
     cases of four operators and returns None for the rest."""
@@ -211,6 +219,10 @@ def fast():
         try:
             from . import _fast as module
         except ImportError:
+            module = None
+        if module is not None and not _fast_is_of_this_process(module):
+            warnings.warn('ferry_b200/_fast.so was built against another torch or Python and is not used; '
+                          'python -m ferry_b200.build builds it anew', RuntimeWarning, stacklevel=2)
             module = None
         if module is None:
             _fast = _NoFast

@@ -266,4 +266,13 @@ PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_fast", nullptr, -1, kMethods, nu
 
 }  // namespace
 
-extern "C" __attribute__((visibility("default"))) PyObject* PyInit__fast() { return PyModule_Create(&kModule); }
+extern "C" __attribute__((visibility("default"))) PyObject* PyInit__fast() {
+  PyObject* m = PyModule_Create(&kModule);
+  // what it was compiled against; _lib.fast() leaves it aside under anything else
+  if (m && (PyModule_AddStringConstant(m, "torch_version", FERRYB_TORCH_VERSION) ||
+            PyModule_AddStringConstant(m, "python_version", PY_VERSION))) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}

@@ -1,11 +1,18 @@
 """The Makefile's rules for the _fast extension, with stand-ins for the
-compilers and the interpreter: no GPU, no nvcc."""
+compilers and the interpreter, and the check of a built one: no GPU, no nvcc."""
 import shutil
 import subprocess
 import sys
+import types
+import warnings
 from pathlib import Path
 
 import pytest
+import torch
+
+import ferry_b200
+from ferry_b200 import _lib
+
 ROOT = Path(__file__).resolve().parents[1]
 
 
@@ -61,6 +68,18 @@ def test_library_alone_where_the_extension_cannot_be_built(tree, tool):
     assert status == 0 and fast.exists()
 
 
+def test_extension_is_rebuilt_for_another_torch(tree):
+    fast = tree / 'ferry_b200' / '_fast.so'
+    assert _make(tree)[0] == 0
+    (tree / 'torch').write_text('2.1.0\n')
+    assert _make(tree)[0] == 0
+    assert fast.exists() and (tree / 'log').read_text().split().count('_fast.so') == 2
+    # one that can no longer be built does not stay from before
+    (tree / 'torch').write_text('2.2.0\n')
+    status, out = _make(tree, CXX=_script(tree / 'broken', 'exit 1\n'))
+    assert status == 0 and not fast.exists()
+
+
 def _flags(tmp_path, torch_source, include=None):
     """torch_flags.py with a stand-in for torch."""
     (tmp_path / 'torch' / 'utils').mkdir(parents=True)
@@ -85,10 +104,37 @@ class _C: _GLIBCXX_USE_CXX11_ABI = True
 def test_flags_name_the_reason(tmp_path):
     (tmp_path / 'Python.h').write_text('')
     run = _flags(tmp_path / 'a', STUB.format(cuda='12.8'), include=tmp_path)
-    assert run.returncode == 0 and '-ltorch_cuda' in run.stdout, run.stderr
+    assert run.returncode == 0 and '-ltorch_cuda' in run.stdout and '2.0.0+x' in run.stdout, run.stderr
     run = _flags(tmp_path / 'b', STUB.format(cuda=None), include=tmp_path)
     assert run.returncode != 0 and 'CUDA' in run.stderr and not run.stdout
     run = _flags(tmp_path / 'c', STUB.format(cuda='12.8'), include=tmp_path / 'a')
     assert run.returncode != 0 and 'Python.h' in run.stderr and not run.stdout
     run = _flags(tmp_path / 'd', 'raise ImportError("none here")\n', include=tmp_path)
     assert run.returncode != 0 and 'none here' in run.stderr and not run.stdout
+
+
+def _load(monkeypatch, **attributes):
+    module = types.ModuleType('ferry_b200._fast')
+    module.__dict__.update(attributes, init=lambda *entries: None)
+    monkeypatch.setitem(sys.modules, 'ferry_b200._fast', module)
+    monkeypatch.setattr(ferry_b200, '_fast', module, raising=False)
+    monkeypatch.setattr(_lib, '_fast', None)
+    return module, _lib.fast
+
+
+def test_an_extension_of_another_torch_or_python_is_not_used(monkeypatch):
+    python = f'{sys.version_info[0]}.{sys.version_info[1]}.99'  # the last number does not matter
+    module, fast = _load(monkeypatch, torch_version=torch.__version__, python_version=python)
+    with warnings.catch_warnings():
+        warnings.simplefilter('error')
+        assert fast() is module
+    for stale in (dict(torch_version='1.0', python_version=python), dict(),
+                  dict(torch_version=torch.__version__, python_version='2.7.1')):
+        _, fast = _load(monkeypatch, **stale)
+        with pytest.warns(RuntimeWarning, match='another'):
+            assert fast() is _lib._NoFast
+
+
+def test_the_built_extension_is_this_one():
+    assert _lib.fast() is not _lib._NoFast
+    assert _lib.fast().torch_version == torch.__version__
