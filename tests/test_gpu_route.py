@@ -220,3 +220,39 @@ def test_group_sums_that_float32_orders_the_other_way():
     sel, _ = _check(x, 2, bias=torch.tensor([1000.0, -1000.0, 1000.0, -1000.0]), score='sigmoid', n_group=2,
                     topk_group=1, group_score='top2')
     assert sel.tolist() == [[0, 1]]
+
+
+@pytest.mark.parametrize('score', ['softmax', 'sigmoid'])
+def test_group_sum_that_is_not_a_number(score):
+    """+inf and -inf biases in one group: its worth is NaN and ranks last, whichever
+    lanes hold the two."""
+    inf = float('inf')
+    for experts, groups in ((8, 4), (64, 8), (32, 16)):
+        size = experts // groups
+        for one in (0, groups - 1):
+            bias = torch.zeros(experts)
+            bias[one * size:(one + 1) * size] = -inf
+            for at in (0, size - 1):
+                b = bias.clone()
+                b[one * size + at] = inf
+                for kept in (1, 2, groups - 1):
+                    with np.errstate(invalid='ignore'):
+                        _check(_logits(20, experts, experts), 2, bias=b, score=score, n_group=groups, topk_group=kept,
+                               group_score='top2')
+
+
+@pytest.mark.parametrize('score', ['softmax', 'sigmoid'])
+@pytest.mark.parametrize('experts', [1024, 256, 40])
+def test_many_ties_and_one_that_is_not(score, experts):
+    """Rows of equal logits, and such rows with one that is a step of float32 above or
+    below, in the first, the last and a middle place."""
+    one = 0.75
+    x = torch.full((7, experts), one)
+    for i, (at, to) in enumerate([(0, 1.0), (0, 0.0), (experts - 1, 1.0), (experts - 1, 0.0), (experts // 2 + 1, 1.0),
+                                  (experts // 2 + 1, 0.0)]):
+        x[i, at] = torch.nextafter(torch.tensor(one), torch.tensor(to))
+    for topk in (1, 8, 32):
+        sel, _ = _check(x, topk, score=score)
+        assert sel[6].tolist() == list(range(topk))
+        _check(x, topk, score=score, bias=torch.linspace(0, 1, 4).repeat(experts // 4).float())
+    _check(x, 4, score=score, n_group=4, topk_group=2, group_score='top2')
