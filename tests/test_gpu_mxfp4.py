@@ -469,3 +469,66 @@ def test_routed_layer_over_fetched_rows():
     slack += 2.0 ** -8 * (np.abs(total) + slack)
     assert bool((np.abs(y.double().cpu().numpy() - total) <= slack).all())
     engine.close()
+
+
+NARROW = ([1, 0, 20, 2, 33], 256, 128, 3, 40, 4)          # hi and lo parts side by side
+WIDE = ([300, 64, 113], 128, 256, 2, 120, 4)              # one after the other
+LONG_SCALES = ([40, 3, 90], 512, 512, 2, 60, 4)           # scale rows that go through TMA
+
+
+def _assert_only_nan(d, bad, good):
+    err = torch.zeros(1, dtype=torch.int32, device=DEV)
+    got = _run(d, err=err)
+    bad = bad.to(DEV)
+    assert int(err) == 0 and bool(bad.any()) and not bool(bad.all())
+    assert bool(got[bad].isnan().all())
+    assert torch.equal(got[~bad], good[~bad])
+
+
+@pytest.mark.parametrize('case', [NARROW, WIDE, LONG_SCALES], ids=['narrow', 'wide', 'long'])
+def test_a_row_that_is_not_finite_is_nan_and_leaves_the_others(case):
+    """Infinities and NaN in inputs and routing weights, activations that overflow: the
+    routes concerned are NaN in every column, their neighbours in a tile the same bits."""
+    inf, nan = float('inf'), float('nan')
+    d = _layer(*case)
+    good = _run(d)
+    assert bool(good.isfinite().all())
+    row, col = int(d['rows'][len(d['rows']) // 2]), int(d['cols'][len(d['rows']) // 2])
+    for at in (0, 31, 77, d['hidden'] - 1):
+        for value in (inf, -inf, nan):
+            x = d['x'].clone()
+            x[row, at] = value
+            _assert_only_nan(dict(d, x=x), d['rows'] == row, good)
+    for value in (inf, -inf, nan):
+        w = d['w'].clone()
+        w[row, col] = value
+        _assert_only_nan(dict(d, w=w), (d['rows'] == row) & (d['cols'] == col), good)
+    # finite inputs: gate and up near 2^90, their product beyond float32
+    x = d['x'].clone()
+    x[row] = (x[row].float() * 2.0 ** 95).to(BF16)
+    _assert_only_nan(dict(d, x=x), d['rows'] == row, good)
+    # a finite activation times a finite weight
+    x[row] = (d['x'][row].float() * 2.0 ** 40).to(BF16)
+    w = d['w'].clone()
+    w[row] = 2.0 ** 120
+    _assert_only_nan(dict(d, x=x, w=w), d['rows'] == row, good)
+
+
+@pytest.mark.parametrize('case', [NARROW, WIDE, LONG_SCALES], ids=['narrow', 'wide', 'long'])
+@pytest.mark.parametrize('low,high,power', [(62, 66, 60), (190, 194, -70), (40, 200, -80), (5, 9, 118), (120, 134, 0)])
+def test_experts_of_far_scales(case, low, high, power):
+    """Scale bytes far from 127, alike and mixed in a row, under inputs that bring gate and
+    up back near 1 (or below)."""
+    d = _layer(*case, low=low, high=high)
+    d['x'] = (d['x'].float() * 2.0 ** power).to(BF16)
+    _assert_close(_run(d), d)
+
+
+@pytest.mark.parametrize('case', [NARROW, WIDE], ids=['narrow', 'wide'])
+def test_columns_far_apart_in_a_block(case):
+    """Blocks of 32 whose values span 2^20: held to 2^-21 of the largest below 2^-13 of it."""
+    d = _layer(*case)
+    g = torch.Generator().manual_seed(9)
+    d['x'] = (d['x'].float() * torch.exp2(-torch.randint(0, 21, d['x'].shape, generator=g).float())).to(BF16)
+    d['w'] = d['w'] * torch.exp2(-torch.randint(0, 60, d['w'].shape, generator=g).float())
+    _assert_close(_run(d), d)
