@@ -11,6 +11,8 @@ from pathlib import Path
 
 import torch
 
+from ._lib import FerrybError
+
 
 @dataclass(frozen=True)
 class ModelSpec:
@@ -73,7 +75,10 @@ def pack_expert(gate_w, up_w, down_w):
 
 def mxfp4_row_bytes(hidden, intermediate):
     """Bytes of an expert row in MXFP4: 3 * H * I codes of half a byte, then one
-    scale byte for every 32 of them (17 bytes where a bf16 row has 64)."""
+    scale byte for every 32 of them (17 bytes where a bf16 row has 64).  H and I
+    are multiples of 32, so that no block has values of two matrix rows."""
+    if hidden <= 0 or intermediate <= 0 or hidden % 32 or intermediate % 32:
+        raise FerrybError(f'hidden ({hidden}) and intermediate ({intermediate}) must be multiples of 32')
     return 3 * hidden * intermediate // 32 * 17
 
 
@@ -81,6 +86,8 @@ def mxfp4_parts(rows):
     """(codes, scales) of MXFP4 expert rows [..., mxfp4_row_bytes]: views of the
     rows, as ferry_b200.expert_ops.quantize_mxfp4 and dequantize_mxfp4 take
     them.  The codes are in the order of pack_expert's values."""
+    if rows.shape[-1] == 0 or rows.shape[-1] % 17:
+        raise FerrybError(f'a row of {rows.shape[-1]} bytes is not whole blocks of 17')
     split = rows.shape[-1] // 17 * 16
     return rows[..., :split], rows[..., split:]
 
@@ -90,8 +97,11 @@ def pack_expert_mxfp4(gate_w, up_w, down_w):
     quantised in blocks of 32 along H (gate, up) and I (down).  H and I are
     multiples of 32."""
     from .expert_ops import quantize_mxfp4
+    if gate_w.dim() != 2 or up_w.shape != gate_w.shape or down_w.shape != gate_w.shape[::-1]:
+        raise FerrybError(f'gate and up must be [I, H], down [H, I]; got {list(gate_w.shape)}, {list(up_w.shape)}, '
+                          f'{list(down_w.shape)}')
+    out = torch.empty(mxfp4_row_bytes(*down_w.shape), dtype=torch.uint8, device=gate_w.device)
     row = pack_expert(gate_w, up_w, down_w)
-    out = torch.empty(row.numel() // 32 * 17, dtype=torch.uint8, device=row.device)
     quantize_mxfp4(row, out=mxfp4_parts(out))
     return out
 

@@ -247,3 +247,26 @@ def test_route_refuses_a_scaling_beyond_float32(calls, scaling):
     expert_ops.route_experts(torch.zeros(3, 8), 2, scaling=float('inf'))
     expert_ops.route_experts(torch.zeros(3, 8), 2, scaling=-3.4028234663852886e38)
     assert len(calls) == 2
+
+
+def test_packing_refuses_blocks_across_rows(calls):
+    """Blocks of 32 run along H and I: other sizes would share scales between rows."""
+    from ferry_b200.model import pack_expert_mxfp4
+    w = torch.zeros
+    for I, H in ((2, 16), (32, 48), (48, 32), (1, 32), (96, 80)):
+        with pytest.raises(FerrybError, match='multiples of 32'):
+            pack_expert_mxfp4(w(I, H), w(I, H), w(H, I))
+        with pytest.raises(FerrybError, match='multiples of 32'):
+            mxfp4_row_bytes(H, I)
+    for gate, up, down in (((32, 64), (64, 32), (64, 32)), ((32, 64), (32, 64), (32, 64)), ((2048,), (2048,), (2048,))):
+        with pytest.raises(FerrybError, match='gate'):
+            pack_expert_mxfp4(w(gate), w(up), w(down))
+    assert not calls
+    assert pack_expert_mxfp4(w(32, 64), w(32, 64), w(64, 32)).shape == (mxfp4_row_bytes(64, 32),)
+    assert len(calls) == 1
+
+
+def test_parts_of_what_is_no_row():
+    for n in (0, 16, 18, 16 * 17 + 1):
+        with pytest.raises(FerrybError, match='17'):
+            mxfp4_parts(torch.zeros(3, n, dtype=torch.uint8))
