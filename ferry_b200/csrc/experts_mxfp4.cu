@@ -16,11 +16,15 @@
 // parts are multiplied and summed into the same float32 accumulator.  A block's
 // largest value is brought to [2^7, 2^8); hi + lo is then the bf16 number itself
 // down to 2^-6 (2^-13 of the largest) and within 2^-14 (2^-21 of the largest)
-// below that, half the lo part's smallest step of 2^-9 * 2^-4.  The activation
-// times its route's weight, operand of the second product, is stored the same way:
-// hi + lo rounds it to within 2^-9 of its value (bf16: 2^-9), or 2^-21 of its
-// block's largest.  Gate, up and silu stay in float32, the result is rounded to
-// bf16 once.
+// below that, half the lo part's smallest step of 2^-9 * 2^-4.  (Of 2^-115 where the
+// block's largest is less: scale bytes have an end.)  The activation times its route's
+// weight, operand of the second product, is stored the same way: hi + lo rounds it to
+// within 2^-9 of its value, half of what bf16's rounding may take (2^-8), or 2^-21 of
+// its block's largest.  It is the one rounding below 32 bits before the result's: two
+// e4m3 parts are what keeps the weights as they are (a third would be half as many
+// bytes and MMAs again in the second product), and an error of 0.0018 of the result's
+// norm against 0.0017 from its rounding to bf16 alone.  Gate, up and silu stay in
+// float32, the result is rounded to bf16 once.
 //
 // Orientation as in experts.cu: 128 weight rows are the MMA's M side (four times
 // 16 gate rows and the 16 up rows of the same features, so that a feature's gate
@@ -52,7 +56,7 @@
 // which the chain prepare - claim - load - phase 1 - phase 2 without queueing is about
 // 11 (32 experts of 256 x 128 take 11.5); 64 tokens (43 experts, 110 MB) 32.5 us: 8
 // before the first load and after the last store, phase 1 at 5.6 TB/s, about 5 lost in
-// the change of phase and with the last items; 4096 tokens of 8 routes 310 us (371 when
+// the change of phase and with the last items; 4096 tokens of 8 routes 310 us (367 to 377 when
 // it runs on and the power limit brings the clock to 1.5 GHz): 36 for the routes' hi and
 // lo parts (134 MB written), then 1,220 cycles a step whose MMAs take 750: loads are
 // under way for 1,900 cycles (850 alone), 33 bytes a cycle into the SM where tiles that
@@ -105,7 +109,7 @@ static_assert(kMxSmem <= 227 * 1024, "shared memory");
 static_assert(kTilePool / ((kTiles + 2) * 512) >= kBlock, "ring of arranged scales");
 constexpr uint64_t kMxWaitNs = 2000000000ull;  // bound on any wait
 
-// Up to 128 routes of one group.
+// Up to 112 routes of one group (kTileCols, MxHeader's cap).
 struct MxGroup {
   int32_t slot;   // cache slot (0 where the caller's is out of range)
   int32_t start;  // first route
@@ -982,7 +986,12 @@ __global__ void __launch_bounds__(kPrepThreads) mxfp4_prepare_kernel(const MxPre
     // to more loads under way, wide ones read the weights less often (128 experts of
     // 2048 x 768, routes of a group in the mean: 16: 32 at most 36.2 us, 48 36.0, 112
     // 40.2; 24: 50.2, 47.7, 53.2; 43: 72.9, 65.0, 65.9 and 64 63.4; 55: 87.2, 77.9, 74.1
-    // and 64 73.8)
+    // and 64 73.8; groups of uneven sizes, 3: 16 49.9, 32 49.7, 112 60.4; 7: 64.6, 64.1,
+    // 76.9).  Of 64 experts of 2048 x 1408 and 16 of 4096 x 1792 the rule is within 3 % of
+    // the best width for means of 1 to 128, of 64 of 512 x 512 within 5 % but for means
+    // of 3 and 80 (18.7 against 16.2, 32.9 against 30.1).  Experts of a step or two of K
+    // would take narrower ones, their items being latency: 128 of 512 x 128 at 24 19.5
+    // against 16.7 with 32, 32 of 256 x 128 at 56 15.6 against 13.4 with 16.
     const int64_t all = a.starts[a.n_groups] - a.starts[0];
     const int64_t mean = active ? (all + active - 1) / active : 0;
     const int cap = mean <= 4 ? 16 : mean <= 16 ? 32 : mean <= 32 ? 48 : mean <= 56 ? 64 : 112;

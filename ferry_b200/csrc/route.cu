@@ -30,8 +30,8 @@
 // lanes (lpg = the power of two <= 32 / G lanes per group, PER consecutive
 // experts each), so the worth of every group comes out of one log2(lpg) step
 // shuffle over all groups at once.  A lane sorts its keys once (19 compare-exchanges
-// for 8), so that a pick looks at the heads alone.  64 tokens of 128 experts: 2.7 us, a
-// launch (4.1 with every token in 64 bits); 16381 tokens of 256 experts in 8 groups: 18.8
+// for 8), so that a pick looks at the heads alone.  64 tokens of 128 experts: 2.5 us, a
+// launch (4.1 with every token in 64 bits); 16381 tokens of 256 experts in 8 groups: 19
 // us (36; 24.6 with a scan of a lane's keys for each pick), bound by some 900
 // instructions a token, a third of them the picks'.
 #include <cuda_fp16.h>

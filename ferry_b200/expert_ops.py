@@ -184,10 +184,12 @@ def route_experts(logits, topk, *, score='softmax', bias=None, n_group=1, topk_g
     biased score (group_score 'max') or sum of their two largest ('top2')
     stay.  The topk largest biased scores are selected, descending, ties to
     the lower id.  The weights are the unbiased scores, divided by their sum
-    with norm_topk_prob, times `scaling`.  -inf logits mask experts with
+    with norm_topk_prob, times `scaling` (a float32).  -inf logits mask experts with
     softmax (a row of nothing else has weights 0); NaN scores are taken last
     and give NaN weights.  Scores are compared in 64 bits.  At most 1024
-    experts, topk <= 32, n_group <= 32."""
+    experts, topk <= 32, n_group <= 32, and in a group at most 32 * (the power of
+    two <= 32 / n_group) experts: 1024 for one group, 512 for 2, 256 for 3 and 4,
+    128 up to 8, 64 up to 16, 32 above."""
     done = _lib.fast().route_experts(logits, topk, score, bias, n_group, topk_group, group_score, norm_topk_prob,
                                      scaling, weights_dtype)
     if done is not None:
@@ -349,8 +351,8 @@ def execute_experts_mxfp4(cache, input, routing_weights, slots, starts, rows, co
     Sums, gate and up are float32, the result is rounded to bf16 once.  Inputs
     and activations (times the route's weight) go into the products as two e4m3
     numbers each, which hold a bf16 input down to 2^-13 of the largest of its 32
-    neighbours exactly and an activation to bf16's precision; a row that is not
-    finite comes out as NaN.  cache is 32-byte aligned, `out` 4-byte aligned (a
+    neighbours exactly and an activation to a bit more than bf16 does; a row that
+    is not finite comes out as NaN.  cache is 32-byte aligned, `out` 4-byte aligned (a
     contiguous bf16 view that starts at an odd element is refused).  Index errors
     are found on the device: the routes' rows become NaN (starts out of order: no
     row is written).  Without `err` the call waits for the GPU and raises; with

@@ -180,13 +180,14 @@ FERRYB_API int ferryb_dequantize_mxfp4(const void* codes, int64_t codes_stride, 
  * The operands x and (silu(x Wg^T) * (x Wu^T)) * weight are held as the sum of
  * two e4m3 numbers with a shared power of two for 32 of them: x exactly down to
  * 2^-13 of the largest of its 32 and within 2^-21 of that below, the second
- * within 2^-9 of its value (bf16's half step) or 2^-21 of the largest; gate and
- * up are float32.  A row whose x or whose activation is not finite comes out as
- * NaN.
+ * within 2^-9 of its value (half of bf16's half step, 2^-8) or 2^-21 of the
+ * largest (of 2^-115 where the largest is less); gate and up are float32.  A row
+ * whose x, or whose activation times its weight, is not finite in float32 comes
+ * out as NaN.
  * Errors found on the device set *err (4, if it was 0) and go on: a row, column
  * or slot out of range makes its routes' outputs NaN; with starts out of order
- * or range no row is written.  *err = 1: a wait inside the kernel ran out, no
- * output is valid.
+ * or range no row is written.  *err = 1: a wait inside the kernel ran out, *err =
+ * 5: its shared memory was not placed as it needs it; no output is valid then.
  * hidden and intermediate: multiples of 128, at most 65536.  The workspace is
  * 256-byte aligned, not shared by calls that may overlap. */
 typedef struct ferryb_mxfp4_experts_args {
