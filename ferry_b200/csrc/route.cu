@@ -512,6 +512,12 @@ extern "C" int ferryb_route_experts(const ferryb_route_args* r, cudaStream_t str
   FB_CHECK_ARG(r->row_stride >= r->experts || r->tokens <= 1, "route_experts: rows overlap");
   if (r->tokens == 0) return FERRYB_OK;
   FB_CHECK_ARG(r->logits && r->selected && r->weights, "route_experts: null pointer");
+  auto whole = [](const void* p, int32_t type) {
+    return reinterpret_cast<uintptr_t>(p) % (type == FERRYB_FP32 ? 4 : 2) == 0;
+  };
+  FB_CHECK_ARG(whole(r->logits, r->logits_type) && whole(r->weights, r->weights_type) &&
+                   whole(r->bias, FERRYB_FP32) && reinterpret_cast<uintptr_t>(r->selected) % 8 == 0,
+               "route_experts: logits, bias, selected and weights must be aligned to their elements");
   a.logits = r->logits;
   a.tokens = r->tokens;
   a.row_stride = r->row_stride;

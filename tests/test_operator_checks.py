@@ -270,3 +270,11 @@ def test_parts_of_what_is_no_row():
     for n in (0, 16, 18, 16 * 17 + 1):
         with pytest.raises(FerrybError, match='17'):
             mxfp4_parts(torch.zeros(3, n, dtype=torch.uint8))
+
+
+@pytest.mark.parametrize('change', [dict(logits=0x1002), dict(logits=0x1001, logits_type=0), dict(bias=0x1002),
+                                    dict(selected=0x1004), dict(weights=0x1001), dict(weights=0x1002, weights_type=2)],
+                         ids=str)
+def test_route_entry_refuses_misaligned_pointers(change):
+    assert _route_status(**change) == 1
+    assert b'aligned' in _lib.lib().ferryb_last_error()
